@@ -5,7 +5,7 @@
 // whose result it reads `every` loads later:
 //   A = 0 no atomic                         A = 1 agent scope, returning, one address per 16 workgroups       A = 2 workgroup scope (performed at the XCD's L2), returning, one address per XCD
 //   A = 3 agent scope, returning, an address per wave (no contention)        A = 4 agent scope, NOT returning, shared address
-//   A = 5 scalar s_atomic_add glc, one address per XCD                      A = 6 system scope, returning, one address per 16 workgroups
+//   A = 6 system scope, returning, one address per 16 workgroups
 //   A = 7 / 8 no atomic, but every wave walks its own span / 8 KB runs (what a wave-level claim makes of the stream) instead of the workgroup's waves side by side, 1 KB each
 // build: hipcc --offload-arch=gfx950 -O3 -o tools/exp/bin/atomic_bubble tools/exp/atomic_bubble.hip
 #include <hip/hip_runtime.h>
@@ -39,12 +39,11 @@ __global__ __launch_bounds__(1024) void bubble_kernel(const u4* __restrict__ src
     asm volatile("v_mov_b32 %0, 0" : "=v"(opaque_zero));
     uint32_t* p;
     if (A == 1 || A == 4 || A == 6) p = ctr + (blockIdx.x / 16) * 64;// 256-byte apart
-    else if (A == 2 || A == 5) p = ctr + xcc * 64;
+    else if (A == 2) p = ctr + xcc * 64;
     else
         p = ctr + (blockIdx.x * NW + wave) * 64;
     uint32_t* const pv = p + opaque_zero;
     uint32_t        acc = 0, pend = 0;
-    [[maybe_unused]] uint32_t spend = 0;
     for (size_t s = 0; s + U * EVERY <= steps; s += U * EVERY) {
         if (A == 1 || A == 3) {
             if (lane == 0) pend = __hip_atomic_fetch_add(pv, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -54,10 +53,6 @@ __global__ __launch_bounds__(1024) void bubble_kernel(const u4* __restrict__ src
             if (lane == 0) pend = __hip_atomic_fetch_add(pv, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         } else if (A == 4) {
             if (lane == 0) (void) __hip_atomic_fetch_add(pv, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        } else if (A == 5) {
-            const uint64_t q = ((uint64_t) __builtin_amdgcn_readfirstlane((uint32_t) ((uint64_t) p >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t) (uint64_t) p);
-            spend            = 1;
-            asm volatile("s_atomic_add %0, %1, 0x0 glc" : "+s"(spend) : "s"(q) : "memory");
         }
 #pragma unroll
         for (int e = 0; e < EVERY; ++e) {
@@ -73,9 +68,6 @@ __global__ __launch_bounds__(1024) void bubble_kernel(const u4* __restrict__ src
         if (A == 1 || A == 2 || A == 3 || A == 6) {
             asm volatile("" : "+v"(pend));
             acc += __builtin_amdgcn_readfirstlane(pend);
-        } else if (A == 5) {
-            asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(spend)::"memory");
-            acc += spend;
         }
     }
     if (acc == 0x12345678u) out[1] = acc;
@@ -127,8 +119,6 @@ int main() {
     run<2, 1>(src, bytes, ctr, out, "workgroup scope, returning, address per XCD");
     run<4, 4>(src, bytes, ctr, out, "agent scope, not returning, address per 16 workgroups");
     run<6, 4>(src, bytes, ctr, out, "system scope, returning, address per 16 workgroups");
-    run<5, 4>(src, bytes, ctr, out, "scalar s_atomic_add glc, address per XCD");
-    run<5, 1>(src, bytes, ctr, out, "scalar s_atomic_add glc, address per XCD");
     run<7, 4>(src, bytes, ctr, out, "no atomic; every wave walks a contiguous span of its own");
     run<8, 4>(src, bytes, ctr, out, "no atomic; every wave walks 8 KB runs, the workgroup's 16 runs side by side");
     return 0;
