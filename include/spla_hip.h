@@ -398,6 +398,52 @@ int splahip_vec_dense_to_coo_limited(int type, uint32_t n, const void* d_dense, 
 int splahip_vec_coo_to_dense(uint32_t n, uint32_t nvals, const uint32_t* d_idx, const void* d_val, uint32_t fill_bits,
                              void* d_dense, void* stream);
 
+/* ---- panels: products with a routing matrix, the experts' products, the norm over many arrays ---------------------
+ * Operators of a layer of experts and of its training step.  Not in the reference.  A panel is a dense row-major matrix of `panel_type` elements without
+ * gaps between its rows.  A router's choice is a matrix of n_rows tokens x n_experts with per_row entries in every row: d_experts[row * per_row + choice]; an
+ * expert outside [0, n_experts) is no entry (padding).  n_places = n_rows * per_row.  All calls are asynchronous on `stream`, keep nothing between calls and
+ * can be captured into a graph; workspaces are the caller's (one call at a time per workspace).  Sums are kept in fp32 or wider, in a fixed order (the same
+ * result from run to run), and rounded to the panel's type once.  Limits: n_experts <= 2048, n_places < 2^31.
+ *
+ * route_sort     : the entries sorted by expert, stable (the transpose of the routing matrix): d_offsets[e] = entries with an expert below e (n_experts + 1
+ *                  words), d_order[p] = the entry at place p, -1 behind the last; d_place[entry] = its place, -1 if it is none.
+ * route_rows     : d_out[p, :] = w * d_x[row of the entry at p, :] (w = d_weights[entry], or 1 with NULL); the rows behind the last entry become 0.
+ * route_back     : d_out[row, :] = sum of w * d_y[place, :] over the row's entries; 0 for a row without any.  It is route_rows' gradient too.
+ * route_back_grad: d_dy[p, :] = w * d_dout[row, :] (0 behind the last entry), d_dweights[entry] = <d_dout[row, :], d_y[place, :]>, 0 where there is no entry.
+ *                  With d_y = the gradient of route_rows' result and d_dout = its panel, d_dweights is the gradient of route_rows' weights. */
+typedef enum splahip_panel_type {
+    SPLAHIP_PANEL_FLOAT    = 0, /* fp32 */
+    SPLAHIP_PANEL_HALF     = 1, /* fp16 */
+    SPLAHIP_PANEL_BFLOAT16 = 2  /* bf16 */
+} splahip_panel_type;
+size_t splahip_route_sort_workspace(uint32_t n_rows, uint32_t per_row, uint32_t n_experts); /* bytes */
+int splahip_route_sort(uint32_t n_rows, uint32_t per_row, uint32_t n_experts, const int32_t* d_experts, uint32_t* d_offsets, int32_t* d_order, int32_t* d_place,
+                       void* d_workspace, size_t workspace_bytes, void* stream);
+int splahip_route_rows(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t n_experts, uint32_t width, const uint32_t* d_offsets, const int32_t* d_place,
+                       const float* d_weights, const void* d_x, void* d_out, void* stream);
+int splahip_route_back(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t width, const int32_t* d_place, const float* d_weights, const void* d_y, void* d_out,
+                       void* stream);
+int splahip_route_back_grad(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t n_experts, uint32_t width, const uint32_t* d_offsets, const int32_t* d_place,
+                            const float* d_weights, const void* d_y, const void* d_dout, void* d_dy, float* d_dweights, void* stream);
+/* expert_product: with the rows in expert order, d_y[p, :] = d_w[e] d_x[p, :] for p in [d_offsets[e], d_offsets[e + 1]), d_w = [n_experts, n_out, n_in] row-major; the
+ * rows behind the last entry become 0 and are not read.  _dx: d_dx[p, :] = d_w[e]^T d_dy[p, :].  _dw: d_dw[e] = sum of d_dy[p, :] d_x[p, :]^T over the expert's
+ * rows (0 without rows).  fp32 panels are multiplied in full fp32. */
+int splahip_expert_product(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_x,
+                           const void* d_w, void* d_y, void* stream);
+int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_dy,
+                              const void* d_w, void* d_dx, void* stream);
+int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_dy,
+                              const void* d_x, void* d_dw, void* stream);
+/* global_norm: *d_norm = sqrt of the sum of the squares of all elements of all arrays (h_ lists on the host: addresses, lengths in elements, panel types); squares
+ * and sums in 64 bits.  clip_global_norm: h_out[i] = h_arrays[i] * min(1, limit / norm) (h_out[i] may be h_arrays[i]; no other overlap); a norm that is not
+ * finite scales nothing.  norm_given != 0: *d_norm is the norm to use (of arrays on several devices, say) and is read; else it is computed and written.
+ * The workspace (splahip_global_norm_workspace bytes, 8-byte aligned) is not needed when the norm is given. */
+size_t splahip_global_norm_workspace(uint32_t n_arrays, const uint64_t* h_lengths);
+int splahip_global_norm(uint32_t n_arrays, const void* const* h_arrays, const uint64_t* h_lengths, const int* h_types, void* d_workspace, size_t workspace_bytes,
+                        float* d_norm, void* stream);
+int splahip_clip_global_norm(uint32_t n_arrays, const void* const* h_arrays, void* const* h_out, const uint64_t* h_lengths, const int* h_types, float limit,
+                             int norm_given, void* d_workspace, size_t workspace_bytes, float* d_norm, void* stream);
+
 /* name of the kernel variant the call above would launch for these arguments (for profiles / DESIGN.md) */
 const char* splahip_mxv_variant(int type, int op_mult, int op_add, int early_exit);
 const char* splahip_mxv_variant_of(splahip_plan plan, int type, int op_mult, int op_add, int early_exit); /* with the plan's sliced-ELL copy taken into account */

@@ -1,0 +1,378 @@
+// route.hip — products with a routing matrix: rows (tokens) x columns (experts), per_row entries in every row, as a router of a layer of experts hands
+// them over.  Sorting the entries by expert is the transpose of that matrix; bringing rows of a panel into that order and back, with weights, is a
+// product of it with a dense operand of many columns.
+//
+//   splahip_route_sort       offsets[e] = number of entries with an expert below e; order = the entries (row * per_row + choice) by (expert, entry);
+//                            place = order's inverse.  An expert outside [0, n_experts) is no entry: its place is -1, order is -1 behind the last entry.
+//   splahip_route_rows       out[p, :] = w_i x[row(i), :], i = order[p]; rows behind the last entry become 0
+//   splahip_route_back       out[r, :] = sum over the row's entries of w_i y[place_i, :]
+//   splahip_route_back_grad  dy[p, :] = w_i dout[row(i), :], dw_i = <dout[row(i), :], y[place_i, :]>
+//
+// Every sum has a fixed order: results are the same from run to run.
+#include "panel.hpp"
+
+namespace splahip {
+
+    constexpr uint32_t kMaxExperts = 2048;
+
+    // ---- the sort: a stable counting sort ------------------------------------------------------------------------------------------------------------
+    // A workgroup owns kSortTile consecutive entries, each of its four wavefronts a quarter of them.  Entry i's position is
+    //   offsets[e] + (entries of e in earlier tiles) + (in earlier wavefronts of the tile) + (in earlier steps of the wavefront) + (in lower lanes of the step),
+    // the last by a ballot per bit of the expert's number.
+    constexpr uint32_t kSortThreads = 256, kSortWaves = kSortThreads / 64, kSortTile = 2048, kSortSteps = kSortTile / kSortThreads;
+
+    __device__ __forceinline__ uint64_t lanes_alike(uint32_t key, bool valid, uint32_t bits) {
+        uint64_t m = __ballot(valid);
+        for (uint32_t b = 0; b < bits; ++b) {
+            const uint64_t with = __ballot((key >> b) & 1u);
+            m &= ((key >> b) & 1u) ? with : ~with;
+        }
+        return m;
+    }
+
+    __global__ __launch_bounds__(256) void route_count_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t n_tiles, const int32_t* __restrict__ experts,
+                                                              uint32_t* __restrict__ counts) {
+        extern __shared__ uint32_t hist[];
+        for (uint32_t e = threadIdx.x; e < n_experts; e += kSortThreads) hist[e] = 0;
+        __syncthreads();
+        for (uint32_t s = 0; s < kSortSteps; ++s) {
+            const uint32_t i = blockIdx.x * kSortTile + s * kSortThreads + threadIdx.x;
+            if (i < n_entries) {
+                const uint32_t e = (uint32_t) experts[i];
+                if (e < n_experts) atomicAdd(&hist[e], 1u);
+            }
+        }
+        __syncthreads();
+        for (uint32_t e = threadIdx.x; e < n_experts; e += kSortThreads) counts[(size_t) e * n_tiles + blockIdx.x] = hist[e];
+    }
+
+    // exclusive scan of one value per thread over the workgroup; total returned through `sum`
+    template<uint32_t THREADS>
+    __device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* sum) {
+        __shared__ uint32_t wave_sum[THREADS / 64];
+        const uint32_t      lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        uint32_t            inc = x;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(inc, d);
+            if (lane >= (uint32_t) d) inc += up;
+        }
+        if (lane == 63) wave_sum[wave] = inc;
+        __syncthreads();
+        uint32_t before = 0, all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < THREADS / 64; ++w) {
+            if (w < wave) before += wave_sum[w];
+            all += wave_sum[w];
+        }
+        __syncthreads();
+        *sum = all;
+        return before + inc - x;
+    }
+
+    // one workgroup per expert: its tiles' counts become exclusive prefixes, their sum the expert's total
+    __global__ __launch_bounds__(256) void route_scan_kernel(uint32_t n_tiles, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
+        uint32_t* mine = counts + (size_t) blockIdx.x * n_tiles;
+        uint32_t  base = 0;
+        for (uint32_t t0 = 0; t0 < n_tiles; t0 += 256) {
+            const uint32_t t = t0 + threadIdx.x;
+            const uint32_t c = t < n_tiles ? mine[t] : 0u;
+            uint32_t       all;
+            const uint32_t ex = block_exclusive<256>(c, &all);
+            if (t < n_tiles) mine[t] = base + ex;
+            base += all;
+        }
+        if (threadIdx.x == 0) totals[blockIdx.x] = base;
+    }
+
+    // positions of the tile's entries; base[e] (LDS) = where the tile's first entry of e goes.  `waves` x n_experts words of LDS behind it.
+    __device__ __forceinline__ void place_tile(uint32_t tile, uint32_t n_entries, uint32_t n_experts, uint32_t bits, const int32_t* __restrict__ experts,
+                                               int32_t* __restrict__ order, int32_t* __restrict__ place, const uint32_t* base, uint32_t* wave_count, uint32_t n_waves,
+                                               uint32_t steps) {
+        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        uint32_t*      mine  = wave_count + wave * n_experts;
+        const uint32_t first = tile * n_waves * steps * 64 + wave * steps * 64;
+        for (uint32_t e = lane; e < n_experts; e += 64) mine[e] = 0;
+        __syncthreads();
+        for (uint32_t s = 0; s < steps; ++s) {
+            const uint32_t i = first + s * 64 + lane;
+            const uint32_t e = i < n_entries ? (uint32_t) experts[i] : ~0u;
+            if (e < n_experts) atomicAdd(&mine[e], 1u);
+        }
+        __syncthreads();
+        // the wavefronts' counts -> where each wavefront's first entry of e goes
+        for (uint32_t e = threadIdx.x; e < n_experts; e += blockDim.x) {
+            uint32_t at = base[e];
+            for (uint32_t w = 0; w < n_waves; ++w) {
+                const uint32_t c               = wave_count[w * n_experts + e];
+                wave_count[w * n_experts + e] = at;
+                at += c;
+            }
+        }
+        __syncthreads();
+        for (uint32_t s = 0; s < steps; ++s) {// (the wavefront's own words only: its LDS accesses stay in program order)
+            const uint32_t i     = first + s * 64 + lane;
+            const uint32_t e     = i < n_entries ? (uint32_t) experts[i] : ~0u;
+            const bool     valid = e < n_experts;
+            const uint64_t alike = lanes_alike(e, valid, bits);
+            const uint32_t below = __popcll(alike & ((1ull << lane) - 1ull));
+            uint32_t       p     = 0;
+            if (valid) p = *(volatile uint32_t*) &mine[e] + below;
+            if (i < n_entries) place[i] = valid ? (int32_t) p : -1;
+            if (valid) {
+                order[p] = (int32_t) i;
+                if (below == 0) *(volatile uint32_t*) &mine[e] = p + (uint32_t) __popcll(alike);
+            }
+        }
+    }
+
+    __global__ __launch_bounds__(256) void route_place_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t n_tiles, uint32_t bits, const int32_t* __restrict__ experts,
+                                                              const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals, uint32_t* __restrict__ offsets,
+                                                              int32_t* __restrict__ order, int32_t* __restrict__ place) {
+        extern __shared__ uint32_t lds[];
+        uint32_t*                  base = lds;// n_experts
+        uint32_t                   run  = 0;
+        for (uint32_t e0 = 0; e0 < n_experts; e0 += kSortThreads) {
+            const uint32_t e = e0 + threadIdx.x;
+            uint32_t       all;
+            const uint32_t at = run + block_exclusive<kSortThreads>(e < n_experts ? totals[e] : 0u, &all);
+            if (e < n_experts) {
+                base[e] = at + counts[(size_t) e * n_tiles + blockIdx.x];
+                if (blockIdx.x == 0) offsets[e] = at;
+            }
+            run += all;
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) offsets[n_experts] = run;
+        // order behind the last entry: this tile's share of those places
+        for (uint32_t s = 0; s < kSortSteps; ++s) {
+            const uint32_t i = blockIdx.x * kSortTile + s * kSortThreads + threadIdx.x;
+            if (i < n_entries && i >= run) order[i] = -1;
+        }
+        __syncthreads();
+        place_tile(blockIdx.x, n_entries, n_experts, bits, experts, order, place, base, lds + n_experts, kSortWaves, kSortSteps);
+    }
+
+    // ---- panels ----------------------------------------------------------------------------------------------------------------------------------------
+    // A row is served by `lanes` neighbouring threads (a power of two, 16 bytes each per step).  All of it is streaming: bound by HBM.
+    struct RowShape {
+        uint32_t lanes;// threads per row
+        uint32_t shift;// log2
+    };
+    static RowShape row_shape(uint32_t units) {
+        RowShape r{1, 0};
+        while (r.lanes < 256 && r.lanes < units) r.lanes <<= 1, ++r.shift;
+        return r;
+    }
+
+    // x is read once and written to each of the row's places (4 rows of the panel would otherwise be fetched from as many distant places of the order).
+    template<typename T, bool WEIGHTED>
+    __global__ __launch_bounds__(256) void route_rows_kernel(uint32_t n_rows, uint32_t per_row, uint32_t width, uint32_t n_experts, uint32_t row_blocks, uint32_t shift,
+                                                             const uint32_t* __restrict__ offsets, const int32_t* __restrict__ place, const float* __restrict__ weights,
+                                                             const T* __restrict__ x, T* __restrict__ out) {
+        constexpr uint32_t U        = kUnit<T>;
+        const uint32_t     lanes    = 1u << shift, sub = threadIdx.x & (lanes - 1u);
+        const uint32_t     n_places = n_rows * per_row;
+        const uint32_t     rows     = 256u >> shift;
+        if (blockIdx.x >= row_blocks) {// the rows behind the last entry
+            const uint32_t end = min(offsets[n_experts], n_places);
+            for (uint64_t p = (uint64_t) end + (blockIdx.x - row_blocks) * rows + (threadIdx.x >> shift); p < n_places; p += (uint64_t) (gridDim.x - row_blocks) * rows)
+                for (uint32_t c = sub * U; c < width; c += lanes * U) {
+                    const float zero[U] = {};
+                    store_unit<T>(out + p * width + c, width - c, zero);
+                }
+            return;
+        }
+        const uint32_t r = blockIdx.x * rows + (threadIdx.x >> shift);
+        if (r >= n_rows) return;
+        for (uint32_t c = sub * U; c < width; c += lanes * U) {
+            float v[U];
+            load_unit<T>(x + (size_t) r * width + c, width - c, v);
+            for (uint32_t j = 0; j < per_row; ++j) {
+                const uint32_t i = r * per_row + j;
+                const uint32_t p = (uint32_t) place[i];
+                if (p >= n_places) continue;
+                if (WEIGHTED) {
+                    const float w = weights[i];
+                    float       s[U];
+#pragma unroll
+                    for (uint32_t q = 0; q < U; ++q) s[q] = w * v[q];
+                    store_unit<T>(out + (size_t) p * width + c, width - c, s);
+                } else {
+                    store_unit<T>(out + (size_t) p * width + c, width - c, v);
+                }
+            }
+        }
+    }
+
+    template<typename T, bool WEIGHTED>
+    __global__ __launch_bounds__(256) void route_back_kernel(uint32_t n_rows, uint32_t per_row, uint32_t width, uint32_t shift, const int32_t* __restrict__ place,
+                                                             const float* __restrict__ weights, const T* __restrict__ y, T* __restrict__ out) {
+        constexpr uint32_t U        = kUnit<T>;
+        const uint32_t     lanes    = 1u << shift, sub = threadIdx.x & (lanes - 1u);
+        const uint32_t     n_places = n_rows * per_row;
+        const uint32_t     r        = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
+        if (r >= n_rows) return;
+        for (uint32_t c = sub * U; c < width; c += lanes * U) {
+            float s[U] = {};
+            for (uint32_t j = 0; j < per_row; ++j) {
+                const uint32_t i = r * per_row + j;
+                const uint32_t p = (uint32_t) place[i];
+                if (p >= n_places) continue;// (no entry: its weight does not count either)
+                float v[U];
+                load_unit<T>(y + (size_t) p * width + c, width - c, v);
+                const float w = WEIGHTED ? weights[i] : 1.0f;
+#pragma unroll
+                for (uint32_t q = 0; q < U; ++q) s[q] = WEIGHTED ? fmaf(w, v[q], s[q]) : s[q] + v[q];
+            }
+            store_unit<T>(out + (size_t) r * width + c, width - c, s);
+        }
+    }
+
+    // one wavefront per row: the products of the entry's weight are reduced inside it
+    template<typename T>
+    __global__ __launch_bounds__(256) void route_back_grad_kernel(uint32_t n_rows, uint32_t per_row, uint32_t width, uint32_t n_experts, uint32_t row_blocks,
+                                                                  const uint32_t* __restrict__ offsets, const int32_t* __restrict__ place,
+                                                                  const float* __restrict__ weights, const T* __restrict__ y, const T* __restrict__ dout,
+                                                                  T* __restrict__ dy, float* __restrict__ dweights) {
+        constexpr uint32_t U        = kUnit<T>;
+        const uint32_t     lane     = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        const uint32_t     n_places = n_rows * per_row;
+        if (blockIdx.x >= row_blocks) {
+            const uint32_t end = min(offsets[n_experts], n_places);
+            for (uint64_t p = (uint64_t) end + (blockIdx.x - row_blocks) * 4 + wave; p < n_places; p += (uint64_t) (gridDim.x - row_blocks) * 4)
+                for (uint32_t c = lane * U; c < width; c += 64 * U) {
+                    const float zero[U] = {};
+                    store_unit<T>(dy + p * width + c, width - c, zero);
+                }
+            return;
+        }
+        const uint32_t r = blockIdx.x * 4 + wave;
+        if (r >= n_rows) return;
+        for (uint32_t j = 0; j < per_row; ++j) {
+            const uint32_t i   = r * per_row + j;
+            const uint32_t p   = (uint32_t) place[i];
+            float          dot = 0.0f;
+            if (p < n_places) {
+                const float w = weights[i];
+                for (uint32_t c = lane * U; c < width; c += 64 * U) {
+                    float g[U], v[U];
+                    load_unit<T>(dout + (size_t) r * width + c, width - c, g);
+                    load_unit<T>(y + (size_t) p * width + c, width - c, v);
+#pragma unroll
+                    for (uint32_t q = 0; q < U; ++q) dot = fmaf(g[q], v[q], dot);
+#pragma unroll
+                    for (uint32_t q = 0; q < U; ++q) g[q] *= w;
+                    store_unit<T>(dy + (size_t) p * width + c, width - c, g);
+                }
+#pragma unroll
+                for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
+            }
+            if (lane == 0) dweights[i] = dot;
+        }
+    }
+
+    static int check_route(uint32_t n_rows, uint32_t per_row, uint32_t n_experts) {
+        SPLAHIP_REQUIRE(per_row >= 1, "entries per row: at least one");
+        SPLAHIP_REQUIRE(n_experts >= 1 && n_experts <= kMaxExperts, "experts: 1 .. 2048");
+        SPLAHIP_REQUIRE((uint64_t) n_rows * per_row < (1ull << 31), "rows x entries per row: below 2^31");
+        return SPLAHIP_OK;
+    }
+    static int check_width(uint32_t width) {
+        SPLAHIP_REQUIRE(width < (1u << 30), "width: below 2^30");
+        return SPLAHIP_OK;
+    }
+    constexpr uint32_t kTailBlocks = 128;// workgroups that clear the rows behind the last entry (none of them: they return at once)
+
+}// namespace splahip
+
+using namespace splahip;
+
+extern "C" size_t splahip_route_sort_workspace(uint32_t n_rows, uint32_t per_row, uint32_t n_experts) {
+    const size_t tiles = ((size_t) n_rows * per_row + kSortTile - 1) / kSortTile;
+    return ((size_t) n_experts * tiles + n_experts) * 4;
+}
+
+extern "C" int splahip_route_sort(uint32_t n_rows, uint32_t per_row, uint32_t n_experts, const int32_t* d_experts, uint32_t* d_offsets, int32_t* d_order,
+                                  int32_t* d_place, void* d_workspace, size_t workspace_bytes, void* stream) {
+    if (int st = check_route(n_rows, per_row, n_experts)) return st;
+    const uint32_t n     = n_rows * per_row;
+    const uint32_t tiles = (n + kSortTile - 1) / kSortTile;
+    SPLAHIP_REQUIRE(d_offsets && (n == 0 || (d_experts && d_order && d_place)), "null array");
+    SPLAHIP_REQUIRE(workspace_bytes >= splahip_route_sort_workspace(n_rows, per_row, n_experts) && d_workspace, "workspace too small");
+    if (int st = ensure_device()) return st;
+    hipStream_t s    = as_stream(stream);
+    uint32_t    bits = 0;
+    while ((1u << bits) < n_experts) ++bits;
+    uint32_t* counts = static_cast<uint32_t*>(d_workspace);
+    uint32_t* totals = counts + (size_t) n_experts * tiles;
+    if (tiles) route_count_kernel<<<tiles, kSortThreads, n_experts * 4, s>>>(n, n_experts, tiles, d_experts, counts);
+    route_scan_kernel<<<n_experts, 256, 0, s>>>(tiles, counts, totals);
+    route_place_kernel<<<tiles ? tiles : 1, kSortThreads, n_experts * 4 * (1 + kSortWaves), s>>>(n, n_experts, tiles, bits, d_experts, counts, totals, d_offsets, d_order, d_place);
+    SPLAHIP_TRY(hipGetLastError());
+    return SPLAHIP_OK;
+}
+
+extern "C" int splahip_route_rows(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t n_experts, uint32_t width, const uint32_t* d_offsets,
+                                  const int32_t* d_place, const float* d_weights, const void* d_x, void* d_out, void* stream) {
+    if (int st = check_route(n_rows, per_row, n_experts)) return st;
+    if (int st = check_width(width)) return st;
+    SPLAHIP_REQUIRE(panel_type_valid(panel_type), "panel type");
+    if (n_rows == 0 || width == 0) return SPLAHIP_OK;
+    SPLAHIP_REQUIRE(d_offsets && d_place && d_x && d_out, "null array");
+    if (int st = ensure_device()) return st;
+    hipStream_t s = as_stream(stream);
+    panel_dispatch(panel_type, [&](auto zero) {
+        using T              = decltype(zero);
+        const RowShape sh    = row_shape((width + kUnit<T> - 1) / kUnit<T>);
+        const uint32_t rows  = 256u >> sh.shift, blocks = (n_rows + rows - 1) / rows;
+        auto*          x     = static_cast<const T*>(d_x);
+        auto*          out   = static_cast<T*>(d_out);
+        if (d_weights) route_rows_kernel<T, true><<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, sh.shift, d_offsets, d_place, d_weights, x, out);
+        else
+            route_rows_kernel<T, false><<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, sh.shift, d_offsets, d_place, d_weights, x, out);
+    });
+    SPLAHIP_TRY(hipGetLastError());
+    return SPLAHIP_OK;
+}
+
+extern "C" int splahip_route_back(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t width, const int32_t* d_place, const float* d_weights, const void* d_y,
+                                  void* d_out, void* stream) {
+    if (int st = check_route(n_rows, per_row, 1)) return st;
+    if (int st = check_width(width)) return st;
+    SPLAHIP_REQUIRE(panel_type_valid(panel_type), "panel type");
+    if (n_rows == 0 || width == 0) return SPLAHIP_OK;
+    SPLAHIP_REQUIRE(d_place && d_y && d_out, "null array");
+    if (int st = ensure_device()) return st;
+    hipStream_t s = as_stream(stream);
+    panel_dispatch(panel_type, [&](auto zero) {
+        using T             = decltype(zero);
+        const RowShape sh   = row_shape((width + kUnit<T> - 1) / kUnit<T>);
+        const uint32_t rows = 256u >> sh.shift, blocks = (n_rows + rows - 1) / rows;
+        auto*          y    = static_cast<const T*>(d_y);
+        auto*          out  = static_cast<T*>(d_out);
+        if (d_weights) route_back_kernel<T, true><<<blocks, 256, 0, s>>>(n_rows, per_row, width, sh.shift, d_place, d_weights, y, out);
+        else
+            route_back_kernel<T, false><<<blocks, 256, 0, s>>>(n_rows, per_row, width, sh.shift, d_place, d_weights, y, out);
+    });
+    SPLAHIP_TRY(hipGetLastError());
+    return SPLAHIP_OK;
+}
+
+extern "C" int splahip_route_back_grad(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t n_experts, uint32_t width, const uint32_t* d_offsets,
+                                       const int32_t* d_place, const float* d_weights, const void* d_y, const void* d_dout, void* d_dy, float* d_dweights, void* stream) {
+    if (int st = check_route(n_rows, per_row, n_experts)) return st;
+    if (int st = check_width(width)) return st;
+    SPLAHIP_REQUIRE(panel_type_valid(panel_type), "panel type");
+    if (n_rows == 0) return SPLAHIP_OK;
+    SPLAHIP_REQUIRE(d_offsets && d_place && d_weights && d_dweights && (width == 0 || (d_y && d_dout && d_dy)), "null array");
+    if (int st = ensure_device()) return st;
+    hipStream_t    s      = as_stream(stream);
+    const uint32_t blocks = (n_rows + 3) / 4;
+    panel_dispatch(panel_type, [&](auto zero) {
+        using T = decltype(zero);
+        route_back_grad_kernel<T><<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, d_offsets, d_place, d_weights, static_cast<const T*>(d_y),
+                                                                       static_cast<const T*>(d_dout), static_cast<T*>(d_dy), d_dweights);
+    });
+    SPLAHIP_TRY(hipGetLastError());
+    return SPLAHIP_OK;
+}

@@ -246,3 +246,235 @@ def mxm(t, a_rows, b_cols, A, B, op_mult, op_add, init, block_products=0, adopt=
               binop_id(op_mult), binop_id(op_add), scalar_bits(init, tid), int(block_products), current_stream_ptr())
     raw = LibraryCsr(Rp, pj, px, nnz.value)
     return (raw.adopt(t) if adopt else raw), prod.value
+
+
+# ---- panels: products with a routing matrix, the experts' products, the norm over many tensors --------------------------------------------------------------
+# A panel is a contiguous 2-D tensor [rows, width] of float32, float16 or bfloat16.  The calls are asynchronous on the current stream of the tensors' device,
+# record no autograd graph (the gradients have calls of their own) and can be captured into a graph.
+
+_PANEL_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class _OnDevice:
+    """the device of a call's tensors made current for its launches"""
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _checked(name, t, dtype, shape, device=None):
+    """t is a contiguous tensor on the GPU of this type, shape and device, else ValueError; returns its address"""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: a tensor expected, not {type(t).__name__}")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} expected, not {t.dtype} of {tuple(t.shape)}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name}: a tensor on {device or 'the GPU'} expected, not on {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous tensor expected, not one of strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _panel_type(name, t):
+    if not isinstance(t, torch.Tensor) or t.dtype not in _PANEL_TYPE:
+        raise ValueError(f"{name}: a tensor of float32, float16 or bfloat16 expected, not {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    return _PANEL_TYPE[t.dtype]
+
+
+def _width(name, t, rows):
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name}: a panel of {rows} rows expected, not shape {tuple(t.shape)}")
+    return t.shape[1]
+
+
+def _stream_of(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class RoutePlan:
+    """The entries of a routing matrix (n_rows tokens x n_experts, per_row entries a row) sorted by expert (route_sort).
+
+    offsets  int32 [n_experts + 1]     the places of expert e are offsets[e] .. offsets[e + 1]
+    order    int32 [n_rows * per_row]  the entry (row * per_row + choice) at each place, -1 behind the last entry
+    place    int32 [n_rows, per_row]   the place of each entry, -1 for no entry
+    """
+
+    __slots__ = ("offsets", "order", "place", "n_rows", "per_row", "n_experts")
+
+    def __init__(self, offsets: torch.Tensor, order: torch.Tensor, place: torch.Tensor):
+        self.offsets, self.order, self.place = offsets, order, place
+        self.n_rows, self.per_row = place.shape
+        self.n_experts = offsets.numel() - 1
+        _checked("offsets", offsets, torch.int32, (self.n_experts + 1,))
+        _checked("order", order, torch.int32, (self.n_rows * self.per_row,), offsets.device)
+        _checked("place", place, torch.int32, (self.n_rows, self.per_row), offsets.device)
+
+    @property
+    def n_places(self):
+        return self.n_rows * self.per_row
+
+    @property
+    def device(self):
+        return self.offsets.device
+
+
+def route_sort(experts: torch.Tensor, n_experts: int) -> RoutePlan:
+    """Sort a router's choices by expert, stable: experts int32 [n_rows, per_row], any number outside [0, n_experts) meaning no entry (padding)."""
+    if not isinstance(experts, torch.Tensor) or experts.dim() != 2:
+        raise ValueError("experts: an int32 tensor [n_rows, per_row] expected")
+    n_rows, per_row = experts.shape
+    src = _checked("experts", experts, torch.int32, (n_rows, per_row))
+    n_experts, device = int(n_experts), experts.device
+    if not 1 <= n_experts <= 2048 or per_row < 1 or n_rows * per_row >= 1 << 31:
+        raise ValueError(f"route_sort serves 1 .. 2048 experts, at least one entry a row and fewer than 2^31 entries, not {n_experts}, {per_row}, {n_rows * per_row}")
+    with _OnDevice(device):
+        offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
+        order = torch.empty(n_rows * per_row, dtype=torch.int32, device=device)
+        place = torch.empty(n_rows, per_row, dtype=torch.int32, device=device)
+        n_bytes = _lib.call("splahip_route_sort_workspace", n_rows, per_row, n_experts)
+        work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
+        _lib.call("splahip_route_sort", n_rows, per_row, n_experts, src, offsets.data_ptr(), order.data_ptr(), place.data_ptr(), work.data_ptr(), n_bytes,
+                  _stream_of(device))
+    return RoutePlan(offsets, order, place)
+
+
+def _weights(plan, weights):
+    return None if weights is None else _checked("weights", weights, torch.float32, (plan.n_rows, plan.per_row), plan.device)
+
+
+def route_rows(plan: RoutePlan, x: torch.Tensor, weights: torch.Tensor = None) -> torch.Tensor:
+    """The rows of x [n_rows, width] in expert order: out[p] = w * x[row of the entry at p], 0 behind the last entry; weights float32 [n_rows, per_row] or None
+    for 1.  Gradients: dx = route_back(plan, dout, weights), dweights = route_back_grad(plan, dout, weights, x)[1]."""
+    t = _panel_type("x", x)
+    width = _width("x", x, plan.n_rows)
+    src, w = _checked("x", x, x.dtype, (plan.n_rows, width), plan.device), _weights(plan, weights)
+    with _OnDevice(plan.device):
+        out = torch.empty(plan.n_places, width, dtype=x.dtype, device=plan.device)
+        _lib.call("splahip_route_rows", t, plan.n_rows, plan.per_row, plan.n_experts, width, plan.offsets.data_ptr(), plan.place.data_ptr(), w, src, out.data_ptr(),
+                  _stream_of(plan.device))
+    return out
+
+
+def route_back(plan: RoutePlan, y: torch.Tensor, weights: torch.Tensor = None) -> torch.Tensor:
+    """The rows of y [n_places, width], in expert order, summed back: out[row] = sum of w * y[place] over the row's entries, 0 for a row without any."""
+    t = _panel_type("y", y)
+    width = _width("y", y, plan.n_places)
+    src, w = _checked("y", y, y.dtype, (plan.n_places, width), plan.device), _weights(plan, weights)
+    with _OnDevice(plan.device):
+        out = torch.empty(plan.n_rows, width, dtype=y.dtype, device=plan.device)
+        _lib.call("splahip_route_back", t, plan.n_rows, plan.per_row, width, plan.place.data_ptr(), w, src, out.data_ptr(), _stream_of(plan.device))
+    return out
+
+
+def route_back_grad(plan: RoutePlan, y: torch.Tensor, weights: torch.Tensor, dout: torch.Tensor):
+    """The gradients (dy, dweights) of route_back(plan, y, weights): dy[p] = w * dout[row] (0 behind the last entry), dweights = <dout[row], y[place]>."""
+    t = _panel_type("y", y)
+    width = _width("y", y, plan.n_places)
+    src = _checked("y", y, y.dtype, (plan.n_places, width), plan.device)
+    w = _checked("weights", weights, torch.float32, (plan.n_rows, plan.per_row), plan.device)
+    g = _checked("dout", dout, y.dtype, (plan.n_rows, width), plan.device)
+    with _OnDevice(plan.device):
+        dy = torch.empty(plan.n_places, width, dtype=y.dtype, device=plan.device)
+        dweights = torch.empty(plan.n_rows, plan.per_row, dtype=torch.float32, device=plan.device)
+        _lib.call("splahip_route_back_grad", t, plan.n_rows, plan.per_row, plan.n_experts, width, plan.offsets.data_ptr(), plan.place.data_ptr(), w, src, g,
+                  dy.data_ptr(), dweights.data_ptr(), _stream_of(plan.device))
+    return dy, dweights
+
+
+def _matrices(plan, w, dtype):
+    if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.shape[0] != plan.n_experts or w.shape[1] < 1 or w.shape[2] < 1:
+        raise ValueError(f"w: matrices [{plan.n_experts}, n_out, n_in] expected, not {tuple(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__}")
+    return _checked("w", w, dtype, w.shape, plan.device)
+
+
+def expert_product(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    """y[p] = w[e] @ x[p] for the places p of expert e: x [n_places, n_in] in expert order, w [n_experts, n_out, n_in] of the same type.  Rows behind the last
+    entry are not read and become 0."""
+    t, src_w = _panel_type("x", x), _matrices(plan, w, x.dtype)
+    n_out, n_in = w.shape[1:]
+    src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
+    with _OnDevice(plan.device):
+        y = torch.empty(plan.n_places, n_out, dtype=x.dtype, device=plan.device)
+        _lib.call("splahip_expert_product", t, plan.n_places, plan.n_experts, n_in, n_out, plan.offsets.data_ptr(), src, src_w, y.data_ptr(), _stream_of(plan.device))
+    return y
+
+
+def expert_product_grad(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, need=(True, True)):
+    """The gradients (dx, dw) of expert_product(plan, x, w): dx[p] = w[e]^T @ dy[p] (0 behind the last entry), dw[e] = sum of dy[p] x[p]^T over the expert's
+    places (0 for an expert without any).  need: which of the two to compute, None stands in the place of the other."""
+    t, src_w = _panel_type("x", x), _matrices(plan, w, x.dtype)
+    n_out, n_in = w.shape[1:]
+    src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
+    src_dy = _checked("dy", dy, x.dtype, (plan.n_places, n_out), plan.device)
+    dx = dw = None
+    with _OnDevice(plan.device):
+        args, offsets, stream = (t, plan.n_places, plan.n_experts, n_in, n_out), plan.offsets.data_ptr(), _stream_of(plan.device)
+        if need[0]:
+            dx = torch.empty_like(x)
+            _lib.call("splahip_expert_product_dx", *args, offsets, src_dy, src_w, dx.data_ptr(), stream)
+        if need[1]:
+            dw = torch.empty_like(w)
+            _lib.call("splahip_expert_product_dw", *args, offsets, src_dy, src, dw.data_ptr(), stream)
+    return dx, dw
+
+
+def _arrays(name, tensors):
+    """address, length and type lists of the tensors, all on one device"""
+    n = len(tensors)
+    ptrs, lengths, types = (C.c_void_p * n)(), (C.c_uint64 * n)(), (C.c_int * n)()
+    device = None
+    for i, t in enumerate(tensors):
+        types[i] = _panel_type(f"{name}[{i}]", t)
+        device = t.device if device is None else device
+        ptrs[i], lengths[i] = _checked(f"{name}[{i}]", t, t.dtype, t.shape, device), t.numel()
+    return ptrs, lengths, types, device
+
+
+def global_norm(tensors) -> torch.Tensor:
+    """The 2-norm over all elements of all tensors (a list of contiguous float32 / float16 / bfloat16 tensors of any shapes on one device), a float32 scalar on
+    that device.  Squares and sums in 64 bits; the order of the sum is fixed."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("tensors: at least one expected")
+    ptrs, lengths, types, device = _arrays("tensors", tensors)
+    with _OnDevice(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        n_bytes = _lib.call("splahip_global_norm_workspace", len(tensors), lengths)
+        work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
+        _lib.call("splahip_global_norm", len(tensors), ptrs, lengths, types, work.data_ptr(), n_bytes, norm.data_ptr(), _stream_of(device))
+    return norm
+
+
+def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None) -> torch.Tensor:
+    """Scale the tensors by min(1, limit / norm), in place or into the list `out` (same shapes and types), and return the norm before.  A norm that is not finite
+    scales nothing (the caller sees it in the result).  norm: a float32 scalar on the device to use instead (the norm over several devices' tensors, say)."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("tensors: at least one expected")
+    ptrs, lengths, types, device = _arrays("tensors", tensors)
+    out_ptrs = ptrs
+    if out is not None:
+        out = list(out)
+        if len(out) != len(tensors):
+            raise ValueError(f"out: {len(tensors)} tensors expected, not {len(out)}")
+        out_ptrs = (C.c_void_p * len(out))(*[_checked(f"out[{i}]", o, t.dtype, t.shape, device) for i, (o, t) in enumerate(zip(out, tensors))])
+    given = norm is not None
+    with _OnDevice(device):
+        if given:
+            _checked("norm", norm, torch.float32, (), device)
+            work, n_bytes = None, 0
+        else:
+            norm = torch.empty((), dtype=torch.float32, device=device)
+            n_bytes = _lib.call("splahip_global_norm_workspace", len(tensors), lengths)
+            work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
+        _lib.call("splahip_clip_global_norm", len(tensors), ptrs, out_ptrs, lengths, types, float(limit), 1 if given else 0, work.data_ptr() if work is not None else None,
+                  n_bytes, norm.data_ptr(), _stream_of(device))
+    return norm
