@@ -162,6 +162,177 @@ namespace splahip {
                 }
     }
 
+    // ---- 16-bit panels: large tiles -------------------------------------------------------------------------------------------------------------------
+    // A workgroup computes BM x BN of the result, BK = 64 of k per step: both operands' slabs go from global memory straight into LDS (16 bytes per lane, no
+    // registers between), double buffered, and feed v_mfma_f32_16x16x32.  The product is taken transposed (the instruction's rows are the result's columns), so that
+    // a lane holds four neighbouring columns of a result row and stores 8 bytes.
+    //
+    // An operand whose k axis is contiguous in memory lies in LDS as [rows][64 of k], one whose row axis is contiguous as [64 of k][rows] and is read
+    // with the transposing LDS read.  The units (16 bytes) of an LDS row are permuted by an exclusive-or with bits of the row's number so that the lanes of
+    // one read meet different banks; the direct loads write LDS in lane order, so the permutation is in the lanes' global addresses.
+    // Units outside the operand (k beyond the depth, rows beyond the tile) come from a page of zeros.
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+    __device__ const uint4 zero_page[4] = {};
+
+    constexpr uint32_t kDepthStep = 64;
+
+    __device__ __forceinline__ uint32_t swz_rows(uint32_t row) { return row & 7u; }                          // [rows][64 of k]: unit ^= this
+    __device__ __forceinline__ uint32_t swz_depth(uint32_t k) { return (k & 3u) | ((k >> 1) & 4u); }          // [64 of k][rows]: pair of units ^= this
+
+    // 16 bytes per lane from global memory to LDS at dst + 16 lane (dst the same for the whole wavefront).  Written as assembly because the compiler waits for every
+    // such load before the next LDS read of any address; the kernel waits itself, by loads_arrived().  It has no result register: nothing the compiler could reuse early.
+    __device__ __forceinline__ void load_to_lds(const void* src, void* dst) {
+        const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t) (uintptr_t) (__attribute__((address_space(3))) void*) dst);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory", "m0");
+    }
+    template<uint32_t LEFT>
+    __device__ __forceinline__ void loads_arrived() {// all but the last LEFT of this wavefront's loads
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+    }
+
+    // one operand's slab of ROWS x 64: THREADS threads, base = its element (row 0, k 0), stride = elements between rows (k contiguous) or between k (rows contiguous)
+    template<typename T, uint32_t ROWS, uint32_t THREADS, bool DEPTH_CONTIGUOUS>
+    __device__ __forceinline__ void stage(const T* __restrict__ base, uint32_t stride, uint32_t rows, uint32_t depth, uint32_t k0, T* lds) {
+        constexpr uint32_t kUnits = ROWS * kDepthStep / 8;
+        static_assert(kUnits % THREADS == 0, "whole steps");
+        const uint32_t wave_base = threadIdx.x & ~63u;
+#pragma unroll
+        for (uint32_t i = 0; i < kUnits / THREADS; ++i) {
+            const uint32_t u = i * THREADS + threadIdx.x;// the unit's place in LDS
+            const void*    src;
+            if (DEPTH_CONTIGUOUS) {
+                const uint32_t row = u >> 3, k = k0 + (((u & 7u) ^ swz_rows(row)) << 3);
+                src = row < rows && k < depth ? (const void*) (base + (size_t) row * stride + k) : (const void*) zero_page;
+            } else {
+                constexpr uint32_t per = ROWS / 8;
+                const uint32_t     kk = u / per, at = u % per, row = (at ^ (swz_depth(kk) << 1)) << 3, k = k0 + kk;
+                src = row < rows && k < depth ? (const void*) (base + (size_t) k * stride + row) : (const void*) zero_page;
+            }
+            load_to_lds(src, lds + (size_t) (i * THREADS + wave_base) * 8);
+        }
+    }
+
+    // the operand of one v_mfma_f32_16x16x32: lane l holds row r0 + l % 16, k = 8 (l / 16) .. + 7 of the 32 at k0
+    template<typename T, uint32_t ROWS, bool DEPTH_CONTIGUOUS>
+    __device__ __forceinline__ s16x8 operand(const T* lds, uint32_t r0, uint32_t k0) {
+        const uint32_t lane = threadIdx.x & 63u;
+        if (DEPTH_CONTIGUOUS) {
+            const uint32_t row = r0 + (lane & 15u), unit = (k0 >> 3) + (lane >> 4);
+            return *reinterpret_cast<const s16x8*>(lds + (size_t) row * kDepthStep + ((unit ^ swz_rows(row)) << 3));
+        } else {
+            // 16 lanes read 4 of k x 16 rows (8 bytes each) and get them transposed: 4 of k of one row
+            s16x4 part[2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t k = k0 + (lane >> 4) * 8 + h * 4 + ((lane & 15u) >> 2);
+                const uint32_t at = ((r0 >> 4) ^ swz_depth(k)) * 16 + (lane & 3u) * 4;
+                part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (lds + (size_t) k * ROWS + at));
+            }
+            return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+
+    __device__ __forceinline__ f32x4 matrix_step(s16x8 a, s16x8 b, f32x4 c, bf16_t) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x4 matrix_step(s16x8 a, s16x8 b, f32x4 c, fp16_t) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
+    }
+
+    // Workgroup number -> tile: workgroups go round the 8 XCDs, each of which has an L2 of its own; an XCD gets a contiguous run of tiles, and a run
+    // walks the columns of kGroup row tiles side by side, so that the workgroups at work in an XCD share both operands' slabs.
+    struct TileAt {
+        uint32_t row, col;
+    };
+    __device__ __forceinline__ TileAt tile_at(uint32_t block, uint32_t row_tiles, uint32_t col_tiles) {
+        constexpr uint32_t kGroup = 4;
+        const uint32_t     total = row_tiles * col_tiles, per = total / 8, extra = total % 8;
+        const uint32_t     xcd = block % 8, local = block / 8;
+        const uint32_t     id    = xcd * per + min(xcd, extra) + local;
+        const uint32_t     group = id / (kGroup * col_tiles), in = id % (kGroup * col_tiles);
+        const uint32_t     height = min(kGroup, row_tiles - group * kGroup);
+        return TileAt{group * kGroup + in % height, in / height};
+    }
+
+    template<typename T, Form FORM, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN>
+    __global__ __launch_bounds__(WM* WN * 64) void product_tile_kernel(const GeneralArgs g, uint32_t row_tiles, uint32_t col_tiles) {
+        constexpr uint32_t THREADS = WM * WN * 64, TM = BM / WM / 16, TN = BN / WN / 16;
+        constexpr bool     A_DEPTH = FORM != kMatrixGrad, B_DEPTH = FORM == kForward;
+        __shared__ __align__(1024) T As[2][BM * kDepthStep];
+        __shared__ __align__(1024) T Bs[2][BN * kDepthStep];
+        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        const T*       A    = static_cast<const T*>(g.a);
+        const T*       B    = static_cast<const T*>(g.b);
+        T*             C    = static_cast<T*>(g.c);
+        const TileAt   at   = tile_at(blockIdx.x, row_tiles, col_tiles);
+        uint32_t       rows, depth, stride_a, stride_b;
+        const uint32_t n0 = at.col * BN, cols = min(BN, g.n - n0);
+        if (FORM == kMatrixGrad) {
+            const uint32_t per = (g.m + BM - 1) / BM, expert = at.row / per, m0 = at.row % per * BM;
+            const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
+            rows                 = min(BM, g.m - m0);
+            depth                = end > begin ? end - begin : 0u;
+            A += (size_t) begin * g.m + m0;
+            B += (size_t) begin * g.n + n0;
+            C += ((size_t) expert * g.m + m0) * g.n + n0;
+            stride_a = g.m, stride_b = g.n;
+        } else {
+            const RowTile t = find_row_tile(at.row, BM, g.n_experts, g.n_places, g.offsets);
+            if (t.expert > g.n_experts) return;
+            rows  = t.rows;
+            depth = t.expert < g.n_experts ? g.k : 0u;
+            A += (size_t) t.row0 * g.k;
+            if (t.expert < g.n_experts) B += FORM == kForward ? ((size_t) t.expert * g.n + n0) * g.k : (size_t) t.expert * g.n * g.k + n0;
+            C += (size_t) t.row0 * g.n + n0;
+            stride_a = g.k, stride_b = FORM == kForward ? g.k : g.n;
+        }
+        const uint32_t wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+        f32x4          acc[TM][TN] = {};
+        const uint32_t steps       = (depth + kDepthStep - 1) / kDepthStep;
+        if (steps) {
+            stage<T, BM, THREADS, A_DEPTH>(A, stride_a, rows, depth, 0, As[0]);
+            stage<T, BN, THREADS, B_DEPTH>(B, stride_b, cols, depth, 0, Bs[0]);
+        }
+        for (uint32_t s = 0; s < steps; ++s) {
+            loads_arrived<0>();
+            __syncthreads();// every wavefront's part of this step's slabs has arrived, the other buffers have been read
+            if (s + 1 < steps) {
+                stage<T, BM, THREADS, A_DEPTH>(A, stride_a, rows, depth, (s + 1) * kDepthStep, As[(s + 1) & 1]);
+                stage<T, BN, THREADS, B_DEPTH>(B, stride_b, cols, depth, (s + 1) * kDepthStep, Bs[(s + 1) & 1]);
+            }
+            const T *as = As[s & 1], *bs = Bs[s & 1];
+#pragma unroll
+            for (uint32_t kk = 0; kk < kDepthStep; kk += 32) {
+                s16x8 a[TM], b[TN];
+#pragma unroll
+                for (uint32_t i = 0; i < TM; ++i) a[i] = operand<T, BM, A_DEPTH>(as, wm + i * 16, kk);
+#pragma unroll
+                for (uint32_t j = 0; j < TN; ++j) b[j] = operand<T, BN, B_DEPTH>(bs, wn + j * 16, kk);
+#pragma unroll
+                for (uint32_t i = 0; i < TM; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < TN; ++j) acc[i][j] = matrix_step(b[j], a[i], acc[i][j], T{});
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < TM; ++i) {
+            const uint32_t m = wm + i * 16 + (lane & 15u);
+            if (m >= rows) continue;
+#pragma unroll
+            for (uint32_t j = 0; j < TN; ++j) {
+                const uint32_t n = wn + j * 16 + (lane >> 4) * 4;
+                if (n >= cols) continue;// (columns come in eights)
+                typedef T four __attribute__((ext_vector_type(4)));
+                four      v;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] = (T) acc[i][j][q];
+                *reinterpret_cast<four*>(C + (size_t) m * g.n + n) = v;
+            }
+        }
+    }
+
     static int check_product(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out) {
         SPLAHIP_REQUIRE(panel_type_valid(panel_type), "panel type");
         SPLAHIP_REQUIRE(n_experts >= 1 && n_experts <= 2048, "experts: 1 .. 2048");
@@ -170,8 +341,27 @@ namespace splahip {
         return SPLAHIP_OK;
     }
 
+    template<typename T, Form FORM, uint32_t BM, uint32_t BN, uint32_t WM, uint32_t WN>
+    static int launch_tiles(const GeneralArgs& g, hipStream_t s) {
+        const uint64_t col_tiles = (g.n + BN - 1) / BN;
+        const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + BM - 1) / BM) : row_tiles_bound(g.n_places, g.n_experts, BM);
+        SPLAHIP_REQUIRE(col_tiles * row_tiles < (1ull << 31), "too many tiles for one launch");
+        product_tile_kernel<T, FORM, BM, BN, WM, WN><<<(uint32_t) (col_tiles * row_tiles), WM * WN * 64, 0, s>>>(g, (uint32_t) row_tiles, (uint32_t) col_tiles);
+        return SPLAHIP_OK;
+    }
+
     template<Form FORM>
     static int launch_product(int panel_type, const GeneralArgs& g, hipStream_t s) {
+        const bool units = ((uintptr_t) g.a % 16 == 0) && ((uintptr_t) g.b % 16 == 0) && ((uintptr_t) g.c % 16 == 0) && g.n % 8 == 0 && g.k % 8 == 0 && g.m % 8 == 0;
+        int        st    = SPLAHIP_OK;
+        if (panel_type != SPLAHIP_PANEL_FLOAT && units) {
+            if (panel_type == SPLAHIP_PANEL_HALF) st = launch_tiles<fp16_t, FORM, 256, 256, 2, 4>(g, s);
+            else
+                st = launch_tiles<bf16_t, FORM, 256, 256, 2, 4>(g, s);
+            if (st) return st;
+            SPLAHIP_TRY(hipGetLastError());
+            return SPLAHIP_OK;
+        }
         const uint64_t col_tiles = (g.n + 63) / 64;
         const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + 63) / 64) : row_tiles_bound(g.n_places, g.n_experts, 64);
         SPLAHIP_REQUIRE(col_tiles * row_tiles < (1ull << 31), "too many tiles for one launch");
@@ -192,7 +382,7 @@ extern "C" int splahip_expert_product(int panel_type, uint32_t n_places, uint32_
     if (n_places == 0) return SPLAHIP_OK;
     SPLAHIP_REQUIRE(d_offsets && d_x && d_w && d_y, "null array");
     if (int st = ensure_device()) return st;
-    return launch_product<kForward>(panel_type, GeneralArgs{d_x, d_w, d_y, n_places, n_experts, n_places, n_out, n_in, d_offsets}, as_stream(stream));
+    return launch_product<kForward>(panel_type, GeneralArgs{d_x, d_w, d_y, n_places, n_experts, 0, n_out, n_in, d_offsets}, as_stream(stream));
 }
 
 extern "C" int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets,
@@ -201,7 +391,7 @@ extern "C" int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint
     if (n_places == 0) return SPLAHIP_OK;
     SPLAHIP_REQUIRE(d_offsets && d_dy && d_w && d_dx, "null array");
     if (int st = ensure_device()) return st;
-    return launch_product<kRowGrad>(panel_type, GeneralArgs{d_dy, d_w, d_dx, n_places, n_experts, n_places, n_in, n_out, d_offsets}, as_stream(stream));
+    return launch_product<kRowGrad>(panel_type, GeneralArgs{d_dy, d_w, d_dx, n_places, n_experts, 0, n_in, n_out, d_offsets}, as_stream(stream));
 }
 
 extern "C" int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets,
