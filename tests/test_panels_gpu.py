@@ -203,6 +203,32 @@ def test_product_of_any_numbers(rows, k, experts, n_in, n_out, dtype):
     _close(got_dw, dw, sdw * (rows * k * 2 * U), dtype)
 
 
+# enough tiles that the card is full of large ones: ragged ranges, depths that end inside a slab, experts without rows, more experts than a wavefront has lanes
+LARGE = [(6000, 2, 5, 328, 2056), (2600, 2, 70, 136, 2304), (700, 1, 200, 264, 520), (9000, 1, 2, 64, 2048), (3000, 2, 3, 2120, 1288)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,k,experts,n_in,n_out", LARGE)
+def test_large_products_of_whole_numbers(rows, k, experts, n_in, n_out, dtype):
+    """sums below 2^24 are exact in fp32 (and in the reference's fp32 product); values -1, 0, 1 keep fp16 results below its largest value"""
+    plan, order, place, end = _case(rows, k, experts, padding=0.1, seed=13)
+    g = torch.Generator(device="cuda").manual_seed(14)
+    x, w, dy = (torch.randint(-1, 2, s, generator=g, device="cuda").to(dtype) for s in ((rows * k, n_in), (experts, n_out, n_in), (rows * k, n_out)))
+    x[end:] = float("nan")
+    dy[end:] = float("nan")
+    y, dx, dw = torch.zeros(rows * k, n_out, device="cuda"), torch.zeros(rows * k, n_in, device="cuda"), torch.zeros(experts, n_out, n_in, device="cuda")
+    offsets = plan.offsets.tolist()
+    for e, (a, b) in enumerate(zip(offsets, offsets[1:])):
+        if a < b:
+            y[a:b] = x[a:b].float() @ w[e].float().t().contiguous()
+            dx[a:b] = dy[a:b].float() @ w[e].float()
+            dw[e] = dy[a:b].float().t().contiguous() @ x[a:b].float()
+    assert max(float(t.abs().max()) for t in (y, dx, dw)) < 65504
+    assert torch.equal(kernels.expert_product(plan, x, w), y.to(dtype))
+    got_dx, got_dw = kernels.expert_product_grad(plan, x, w, dy)
+    assert torch.equal(got_dx, dx.to(dtype)) and torch.equal(got_dw, dw.to(dtype))
+
+
 def test_product_needs():
     plan, x, w, dy, _ = _product_case(20, 2, 3, 24, 40, torch.float32, True)
     x, w, dy = x.cuda(), w.cuda(), dy.cuda()
