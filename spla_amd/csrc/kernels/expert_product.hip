@@ -6,7 +6,7 @@
 //   splahip_expert_product_dw  dw[e]    = sum over the expert's rows of dy[p, :] x[p, :]^T
 //
 // Rows behind the last entry (offsets[n_experts] ..) become 0; an expert without rows has dw = 0.  fp32 sums in a fixed order, one rounding to the panel's
-// type.  fp32 panels are multiplied in full fp32 (v_mfma_f32_16x16x4_f32).
+// type.  fp32 panels are multiplied in full fp32 (v_mfma_f32_32x32x2_f32).
 #include "panel.hpp"
 #include <type_traits>
 
@@ -14,6 +14,7 @@
 namespace splahip {
 
     typedef float    f32x4 __attribute__((ext_vector_type(4)));
+    typedef float    f32x16 __attribute__((ext_vector_type(16)));
     typedef bf16_t   bf16x8 __attribute__((ext_vector_type(8)));
     typedef fp16_t   fp16x8 __attribute__((ext_vector_type(8)));
 
@@ -57,168 +58,6 @@ namespace splahip {
     // upper bound of the number of row tiles (the host does not know the ranges)
     static uint64_t row_tiles_bound(uint32_t n_places, uint32_t n_experts, uint32_t bm) {
         return n_places / bm + (uint64_t) min(n_experts + 1, n_places);
-    }
-
-    // ---- the general kernel ----------------------------------------------------------------------------------------------------------------------------
-    // C[m, n] = sum over k of A(m, k) B(n, k) for any sizes, strides and alignment: 64 x 64 tiles, 32 of k per step through LDS, element loads with bounds.
-    enum Form { kForward, kRowGrad, kMatrixGrad };
-
-    struct GeneralArgs {
-        const void *a, *b;
-        void*       c;
-        uint32_t    n_places, n_experts, m, n, k;// kForward: n = n_out, k = n_in; kRowGrad: n = n_in, k = n_out; kMatrixGrad: m = n_out, n = n_in
-        const uint32_t* offsets;
-    };
-
-    template<typename T>
-    struct Step;// one 16 x 16 result tile, 32 of k, operands of lane l: row l % 16, k = 8 (l / 16) ..
-    template<>
-    struct Step<bf16_t> {
-        static __device__ __forceinline__ f32x4 mul(const bf16_t* a, const bf16_t* b, f32x4 c) {
-            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(a), *reinterpret_cast<const bf16x8*>(b), c, 0, 0, 0);
-        }
-    };
-    template<>
-    struct Step<fp16_t> {
-        static __device__ __forceinline__ f32x4 mul(const fp16_t* a, const fp16_t* b, f32x4 c) {
-            return __builtin_amdgcn_mfma_f32_16x16x32_f16(*reinterpret_cast<const fp16x8*>(a), *reinterpret_cast<const fp16x8*>(b), c, 0, 0, 0);
-        }
-    };
-    template<>
-    struct Step<float> {// (the order of k inside a step is free as long as both operands share it)
-        static __device__ __forceinline__ f32x4 mul(const float* a, const float* b, f32x4 c) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-            return c;
-        }
-    };
-
-    template<typename T, Form FORM>
-    __global__ __launch_bounds__(256) void product_general_kernel(const GeneralArgs g, uint32_t col_tiles) {
-        constexpr uint32_t BM = 64, BN = 64, BK = 32, LD = BK + kUnit<T>;// (row stride of the LDS tiles: a unit more than BK against bank conflicts)
-        __shared__ __align__(16) T As[BM * LD];
-        __shared__ __align__(16) T Bs[BN * LD];
-        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-        const T*       A    = static_cast<const T*>(g.a);
-        const T*       B    = static_cast<const T*>(g.b);
-        T*             C    = static_cast<T*>(g.c);
-        uint32_t       m0, n0, rows, cols, depth, expert;
-        size_t         sam, sak, sbn, sbk, ldc;// element strides of A(m, k), B(n, k) and C's rows
-        const uint32_t tile = blockIdx.x / col_tiles, col = blockIdx.x % col_tiles;
-        n0 = col * BN;
-        if (FORM == kMatrixGrad) {
-            const uint32_t row_tiles = (g.m + BM - 1) / BM;
-            expert                   = tile / row_tiles;
-            m0                       = tile % row_tiles * BM;
-            rows                     = min(BM, g.m - m0);
-            cols                     = min(BN, g.n - n0);
-            const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
-            depth = end > begin ? end - begin : 0u;
-            A += (size_t) begin * g.m + m0;
-            B += (size_t) begin * g.n + n0;
-            sam = 1, sak = g.m, sbn = 1, sbk = g.n;
-            C += ((size_t) expert * g.m + m0) * g.n + n0;
-        } else {
-            const RowTile t = find_row_tile(tile, BM, g.n_experts, g.n_places, g.offsets);
-            if (t.expert > g.n_experts) return;
-            m0 = t.row0, rows = t.rows, expert = t.expert;
-            cols  = min(BN, g.n - n0);
-            depth = expert < g.n_experts ? g.k : 0u;
-            A += (size_t) m0 * g.k;
-            sam = g.k, sak = 1;
-            if (FORM == kForward) B += ((size_t) expert * g.n + n0) * g.k, sbn = g.k, sbk = 1;
-            else
-                B += (size_t) expert * g.n * g.k + n0, sbn = 1, sbk = g.n;
-            C += (size_t) m0 * g.n + n0;
-        }
-        ldc = g.n;
-        f32x4 acc[2][2] = {};
-        const uint32_t wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-        for (uint32_t k0 = 0; k0 < depth; k0 += BK) {
-            __syncthreads();
-#pragma unroll
-            for (uint32_t s = 0; s < BM * BK / 256; ++s) {
-                const uint32_t i = s * 256 + threadIdx.x;
-                // neighbouring threads along the axis that is contiguous in memory
-                const uint32_t am = FORM == kMatrixGrad ? i % BM : i / BK, ak = FORM == kMatrixGrad ? i / BM : i % BK;
-                const uint32_t bn = FORM == kForward ? i / BK : i % BN, bk = FORM == kForward ? i % BK : i / BN;
-                As[am * LD + ak]  = am < rows && k0 + ak < depth ? A[am * sam + (k0 + ak) * sak] : (T) 0.0f;
-                Bs[bn * LD + bk]  = bn < cols && k0 + bk < depth ? B[bn * sbn + (k0 + bk) * sbk] : (T) 0.0f;
-            }
-            __syncthreads();
-            const uint32_t r = lane & 15u, q = (lane >> 4) * 8;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[i][j] = Step<T>::mul(As + (wm + i * 16 + r) * LD + q, Bs + (wn + j * 16 + r) * LD + q, acc[i][j]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const uint32_t m = wm + i * 16 + (lane >> 4) * 4 + v, n = wn + j * 16 + (lane & 15u);
-                    if (m < rows && n < cols) C[m * ldc + n] = (T) acc[i][j][v];
-                }
-    }
-
-    // ---- 16-bit panels: large tiles -------------------------------------------------------------------------------------------------------------------
-    // A workgroup computes BM x BN of the result, BK = 64 of k per step: both operands' slabs go from global memory straight into LDS (16 bytes per lane, no
-    // registers between), double buffered, and feed v_mfma_f32_16x16x32.  The product is taken transposed (the instruction's rows are the result's columns), so that
-    // a lane holds four neighbouring columns of a result row and stores 8 bytes.
-    //
-    // An operand whose k axis is contiguous in memory lies in LDS as [rows][64 of k], one whose row axis is contiguous as [64 of k][rows] and is read
-    // with the transposing LDS read.  The units (16 bytes) of an LDS row are permuted by an exclusive-or with bits of the row's number so that the lanes of
-    // one read meet different banks; the direct loads write LDS in lane order, so the permutation is in the lanes' global addresses.
-    // Units outside the operand (k beyond the depth, rows beyond the tile) come from a page of zeros.
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef short s16x8 __attribute__((ext_vector_type(8)));
-
-    __device__ const uint4 zero_page[4] = {};
-
-    constexpr uint32_t kDepthStep = 64;
-
-    __device__ __forceinline__ uint32_t swz_rows(uint32_t row) { return (row >> 1) & 7u; }                          // [rows][64 of k]: unit ^= this
-    __device__ __forceinline__ uint32_t swz_depth(uint32_t k) { return (k & 3u) << 1; }          // [64 of k][rows]: pair of units ^= this
-
-    // 16 bytes per lane from global memory to LDS at dst + 16 lane (dst the same for the whole wavefront).  Written as assembly because the compiler waits for every
-    // such load before the next LDS read of any address; the kernel waits itself, by loads_arrived().  It has no result register: nothing the compiler could reuse early.
-    __device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
-    }
-    template<uint32_t LEFT>
-    __device__ __forceinline__ void loads_arrived() {// all but the last LEFT of this wavefront's loads
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
-    }
-
-    // the operand of one v_mfma_f32_32x32x16: lane l holds row r0 + l % 32, k = k0 + 8 (l / 32) .. + 7
-    template<typename T, uint32_t ROWS, bool DEPTH_CONTIGUOUS>
-    __device__ __forceinline__ s16x8 operand(const T* lds, uint32_t r0, uint32_t k0) {
-        const uint32_t lane = threadIdx.x & 63u;
-        if (DEPTH_CONTIGUOUS) {
-            const uint32_t row = r0 + (lane & 31u), unit = (k0 >> 3) + (lane >> 5);
-            return *reinterpret_cast<const s16x8*>(lds + (size_t) row * kDepthStep + ((unit ^ swz_rows(row)) << 3));
-        } else {
-            // 16 lanes read 4 of k x 16 rows (8 bytes each) and get them transposed: 4 of k of one row
-            s16x4 part[2];
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint32_t k  = k0 + (lane >> 5) * 8 + h * 4 + ((lane & 15u) >> 2);
-                const uint32_t at = (((r0 >> 4) + ((lane >> 4) & 1u)) ^ swz_depth(k)) * 16 + (lane & 3u) * 4;
-                part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (lds + (size_t) k * ROWS + at));
-            }
-            return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-    }
-
-    typedef float f32x16 __attribute__((ext_vector_type(16)));
-    __device__ __forceinline__ f32x16 matrix_step(s16x8 a, s16x8 b, f32x16 c, bf16_t) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    }
-    __device__ __forceinline__ f32x16 matrix_step(s16x8 a, s16x8 b, f32x16 c, fp16_t) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
     }
 
     // The row tiles of the first 64 experts stay in a wavefront's registers (lane = expert), so that finding a tile's rows costs no memory access; further ones are found by
@@ -276,78 +115,213 @@ namespace splahip {
         return p;
     }
 
-    // One operand's slab of ROWS x 64 of k, THREADS threads, 16 bytes each per load.  stride = elements between rows (k contiguous) or between k (rows contiguous).  The lane's byte offsets
-    // from the slab's first element are made once per tile; the slab's address moves in scalar registers.  Rows outside the tile read the tile's first row instead (their
-    // results are not stored).
-    template<typename T, uint32_t ROWS, uint32_t THREADS, bool DEPTH_CONTIGUOUS>
+    // C[m, n] = sum over k of A(m, k) B(n, k).  A result tile is a workgroup's; rows of A and B are the result's rows and columns.
+    enum Form { kForward, kRowGrad, kMatrixGrad };
+
+    struct ProductArgs {
+        const void *a, *b;
+        void*       c;
+        uint32_t    n_places, n_experts, m, n, k;// kForward: n = n_out, k = n_in; kRowGrad: n = n_in, k = n_out; kMatrixGrad: m = n_out, n = n_in
+        const uint32_t* offsets;
+    };
+
+    // ---- LDS ---------------------------------------------------------------------------------------------------------------------------------------------
+    // A step of k takes kStep elements (128 bytes).  An operand's slab of a step lies in LDS as [rows][128 bytes of k] if its k axis is contiguous in memory, as
+    // [k][rows] if its rows are.  16-byte units are permuted by an exclusive-or with bits of the LDS row's number: the lanes that LDS serves in one clock (16 of them
+    // at 16 bytes, 256 bytes in all) then meet different banks (no conflict counted in either layout).
+    template<typename T>
+    constexpr uint32_t kStep = 128 / sizeof(T);
+
+    __device__ __forceinline__ uint32_t swz_rows(uint32_t row) { return (row >> 1) & 7u; }
+    template<typename T>
+    __device__ __forceinline__ uint32_t swz_depth(uint32_t k) {
+        return sizeof(T) == 2 ? (k & 3u) << 2 : ((k >> 2) & 1u) << 3;
+    }
+
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));// 16 bytes of any element type
+
+    // What a matrix instruction takes: lane l holds row r0 + l % 32, 16 bytes of k from k0 + (l / 32) * kUnit
+    template<typename T, uint32_t ROWS, bool DEPTH_CONTIGUOUS>
+    __device__ __forceinline__ s16x8 operand(const T* lds, uint32_t r0, uint32_t k0) {
+        const uint32_t lane = threadIdx.x & 63u;
+        if constexpr (DEPTH_CONTIGUOUS) {
+            const uint32_t row = r0 + (lane & 31u), unit = k0 / kUnit<T> + (lane >> 5);
+            return *reinterpret_cast<const s16x8*>(lds + row * kStep<T> + ((unit ^ swz_rows(row)) * kUnit<T>));
+        } else if constexpr (sizeof(T) == 2) {
+            // the transposing read: 16 lanes take 4 of k x 16 rows (8 bytes each) and get 4 of k of one row each
+            static_assert(ROWS >= 128, "the permutation needs 16 units per row");
+            s16x4 part[2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                const uint32_t k = k0 + (lane >> 5) * 8 + h * 4 + ((lane & 15u) >> 2), row = r0 + (lane & 16u) + (lane & 3u) * 4;
+                const uint32_t at = ((row >> 3) ^ swz_depth<T>(k)) * 8 + (row & 7u);
+                part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*) (lds + k * ROWS + at));
+            }
+            return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            const uint32_t row = r0 + (lane & 31u);
+            f32x4          v;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t k = k0 + (lane >> 5) * 4 + i;
+                v[i]             = lds[k * ROWS + (((row >> 2) ^ swz_depth<T>(k)) * 4 + (row & 3u))];
+            }
+            return __builtin_bit_cast(s16x8, v);
+        }
+    }
+
+    // 32 x 32 of the result, two units of k.  fp32: the order of k inside the step is free as long as both operands share it.
+    __device__ __forceinline__ f32x16 matrix_step(s16x8 a, s16x8 b, f32x16 c, bf16_t) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x16 matrix_step(s16x8 a, s16x8 b, f32x16 c, fp16_t) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x16 matrix_step(s16x8 a, s16x8 b, f32x16 c, float) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    }
+
+    // ---- from memory to LDS ------------------------------------------------------------------------------------------------------------------------------
+    // kUnits: 16 bytes per lane straight into LDS; operands, rows and the result begin at multiples of 16 bytes.
+    // kWords: 4 bytes per lane straight into LDS; fp32 of any sizes.
+    // kElements: through registers, 16 bytes per lane from any address, the ends of rows element by element; 16-bit elements of odd sizes or alignment.
+    enum Load { kUnits, kWords, kElements };
+
+    __device__ const uint4 zero_page[4] = {};
+
+    // One load per lane into LDS at dst + (16 or 4) lane, dst the same for the whole wavefront.  Assembly, because the compiler waits for every such load before the next LDS
+    // read of any address; the kernel waits itself, by loads_arrived().  There is no result register that the compiler could reuse early.  (M0 holds dst; the
+    // compiler sets it anew wherever it needs it.)
+    template<Load LOAD>
+    __device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
+        if constexpr (LOAD == kUnits) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+        else
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
+    }
+    template<Load LOAD>
+    __device__ __forceinline__ void load_to_lds_at(const void* base, uint32_t offset, uint32_t dst) {
+        if constexpr (LOAD == kUnits) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+        else
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+    }
+    template<uint32_t LEFT>
+    __device__ __forceinline__ void loads_arrived() {// all but the last LEFT of this wavefront's loads (and stores) into memory order
+        static_assert(LEFT < 64, "a six-bit counter");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+    }
+
+    // One operand's slab: ROWS rows, THREADS threads, kLoads loads each.  stride = elements between rows (k contiguous) or between k (rows contiguous).  The lane's byte
+    // offsets from the slab's first element are made once per tile; the slab's address moves in scalar registers.  Rows outside the tile read the tile's first row
+    // instead: their results are not stored.
+    template<typename T, uint32_t ROWS, uint32_t THREADS, bool DEPTH_CONTIGUOUS, Load LOAD>
     struct Slab {
-        static constexpr uint32_t kLoads = ROWS * 8 / THREADS, kPerDepth = ROWS / 8;
+        static constexpr uint32_t kPiece = LOAD == kWords ? 4 : 16, kLoads = ROWS * 128 / (THREADS * kPiece), kPerDepth = ROWS / kUnit<T>;
+        static __device__ __forceinline__ uint32_t unit(uint32_t i) { return (i * THREADS + threadIdx.x) * kPiece / 16; }
+        static __device__ __forceinline__ uint32_t sub(uint32_t i) { return (i * THREADS + threadIdx.x) * kPiece % 16 / sizeof(T); }
+        // the lane's first k and row inside the slab
+        static __device__ __forceinline__ uint32_t depth_of(uint32_t i) {
+            return DEPTH_CONTIGUOUS ? ((unit(i) & 7u) ^ swz_rows(unit(i) >> 3)) * kUnit<T> + sub(i) : unit(i) / kPerDepth;
+        }
+        static __device__ __forceinline__ uint32_t row_of(uint32_t i) {
+            return DEPTH_CONTIGUOUS ? unit(i) >> 3 : ((unit(i) % kPerDepth) ^ swz_depth<T>(depth_of(i))) * kUnit<T> + sub(i);
+        }
         static __device__ __forceinline__ void offsets(uint32_t stride, uint32_t rows, uint32_t (&off)[kLoads]) {
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const uint32_t u = i * THREADS + threadIdx.x;
-                if (DEPTH_CONTIGUOUS) {
-                    const uint32_t row = u >> 3;
-                    off[i]             = ((row < rows ? row * stride : 0u) + depth_of(i)) * sizeof(T);
-                } else {
-                    const uint32_t kk = depth_of(i), row = ((u % kPerDepth) ^ (swz_depth(kk) << 1)) << 3;
-                    off[i] = (kk * stride + (row < rows ? row : 0u)) * sizeof(T);
+                const uint32_t row = row_of(i) < rows ? row_of(i) : 0u;
+                off[i]             = (DEPTH_CONTIGUOUS ? row * stride + depth_of(i) : depth_of(i) * stride + row) * (uint32_t) sizeof(T);
+            }
+        }
+        static __device__ __forceinline__ void load(const T* base, const uint32_t (&off)[kLoads], uint32_t i, uint32_t dst) {
+            load_to_lds_at<LOAD>(base, off[i], dst + i * (THREADS * kPiece));
+        }
+        // the slab that the depth ends in (left < kStep of it): what lies behind comes from a page of zeros
+        static __device__ __forceinline__ void load_last(const T* base, const uint32_t (&off)[kLoads], uint32_t left, uint32_t dst) {
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i)
+                load_to_lds<LOAD>(depth_of(i) < left ? reinterpret_cast<const char*>(base) + off[i] : reinterpret_cast<const char*>(zero_page), dst + i * (THREADS * kPiece));
+        }
+        // kElements: into registers ..
+        static __device__ __forceinline__ void fetch(const T* base, const uint32_t (&off)[kLoads], uint32_t rows, uint32_t left, s16x8 (&r)[kLoads]) {
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const T*       p   = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off[i]);
+                const uint32_t row = row_of(i) < rows ? row_of(i) : 0u, k = depth_of(i);
+                // elements of the unit that exist: a row of k ends at `left`, a row of rows at `rows`
+                const uint32_t have = DEPTH_CONTIGUOUS ? (k < left ? left - k : 0u) : (k < left ? rows - row : 0u);
+                if (have >= (uint32_t) kUnit<T>) r[i] = __builtin_bit_cast(s16x8, *reinterpret_cast<const typename UnitOf<T>::mem*>(p));
+                else {
+                    T v[kUnit<T>];
+#pragma unroll
+                    for (uint32_t q = 0; q < (uint32_t) kUnit<T>; ++q) v[q] = q < have ? p[q] : (T) 0.0f;
+                    r[i] = *reinterpret_cast<const s16x8*>(v);
                 }
             }
         }
-        // the lane's first k inside the slab
-        static __device__ __forceinline__ uint32_t depth_of(uint32_t i) {
-            const uint32_t u = i * THREADS + threadIdx.x;
-            return DEPTH_CONTIGUOUS ? ((u & 7u) ^ swz_rows(u >> 3)) << 3 : u / kPerDepth;
+        // .. and on into LDS
+        static __device__ __forceinline__ void put(const s16x8 (&r)[kLoads], T* slab) {
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) *reinterpret_cast<s16x8*>(slab + unit(i) * kUnit<T>) = r[i];
         }
     };
-    __device__ __forceinline__ void load_to_lds_at(const void* base, uint32_t offset, uint32_t dst) {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
-    }
 
-    // the slab that the depth ends in: units behind it come from the page of zeros
-    template<typename S, typename T>
-    __device__ __forceinline__ void last_slab(const T* base, const uint32_t (&off)[S::kLoads], uint32_t left, uint32_t dst, uint32_t step) {
+    // ---- the kernel --------------------------------------------------------------------------------------------------------------------------------------
+    // A workgroup stays and computes one BM x BM tile after another, WM x WN wavefronts side by side.  A step of k is four quarters of two units: while a quarter's matrix
+    // instructions run from registers, the operands of the next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last
+    // quarter: behind it every wavefront has read this step's two slabs, so the next two loads may overwrite them, and the next step's slabs have arrived (issued one
+    // step ago, A's two steps ago).  The loads of the next tile's first slabs are under way while a tile's result is stored.
+    // 16 bytes of a result row, or as many of their elements as the row has left
+    template<typename T>
+    __device__ __forceinline__ void store_part(T* p, uint32_t left, s16x8 c) {
+        if (left >= (uint32_t) kUnit<T>) *reinterpret_cast<typename UnitOf<T>::mem*>(p) = __builtin_bit_cast(typename UnitOf<T>::mem, c);
+        else {
+            T v[kUnit<T>];
+            *reinterpret_cast<s16x8*>(v) = c;
 #pragma unroll
-        for (uint32_t i = 0; i < S::kLoads; ++i)
-            load_to_lds(S::depth_of(i) < left ? reinterpret_cast<const char*>(base) + off[i] : reinterpret_cast<const char*>(zero_page), dst + i * step);
+            for (uint32_t q = 0; q < (uint32_t) kUnit<T>; ++q)
+                if (q < left) p[q] = v[q];
+        }
     }
 
-    // A workgroup stays and computes one tile after another.  A step of k (64) is four quarters of 16: while a quarter's matrix instructions run from registers, the operands of the
-    // next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last quarter: behind it every wavefront has read this step's two slabs, so the
-    // next two loads may overwrite them, and the next step's slabs have arrived (issued one step ago, A's two steps ago).  The loads of the next tile's first slabs are
-    // under way while a tile's result is stored.
-    template<typename T, Form FORM, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC>
-    __global__ __launch_bounds__(WM* WN * 64, OCC) void product_tile_kernel(const GeneralArgs g, uint32_t col_tiles) {
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC>
+    __global__ __launch_bounds__(WM* WN * 64, OCC) void product_kernel(const ProductArgs g, uint32_t col_tiles) {
         constexpr uint32_t BN = BM, THREADS = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
-        constexpr uint32_t LOADS = BM * 8 / THREADS;// per thread and slab
         constexpr bool     A_DEPTH = FORM != kMatrixGrad, B_DEPTH = FORM == kForward;
-        using SlabA = Slab<T, BM, THREADS, A_DEPTH>;
-        using SlabB = Slab<T, BN, THREADS, B_DEPTH>;
-        constexpr uint32_t kSlots = 5, kSlab = BM * kDepthStep;
-        constexpr uint32_t kMul = TM * TN, kReads = TM + TN;
-        constexpr uint32_t kCols = BN / WN, kRowUnits = kCols / 8, kStores = TM * 32 * kRowUnits / 64;
+        using SlabA                   = Slab<T, BM, THREADS, A_DEPTH, LOAD>;
+        using SlabB                   = Slab<T, BN, THREADS, B_DEPTH, LOAD>;
+        constexpr uint32_t LOADS      = SlabA::kLoads;// per thread and slab
+        constexpr uint32_t kSlots     = 5, kSlab = BM * kStep<T>;
+        constexpr uint32_t kMul       = TM * TN, kReads = TM + TN, kReadsPer = (kReads + kMul - 1) / kMul, kQuarter = 2 * kUnit<T>;
+        // the result is turned in the fifth slab, 32 rows x kTurn tiles of 32 columns at a time and wavefront
+        constexpr uint32_t kTurn = sizeof(T) == 2 ? TN : 1, kTurnCols = kTurn * 32, kRowUnits = kTurnCols / kUnit<T>;
+        constexpr bool     kTurns = WM * WN * 32 * kTurnCols <= kSlab;
+        constexpr uint32_t kStores = kTurns ? TM * (TN / kTurn) * 32 * kRowUnits / 64 : TM * TN * 4;
         __shared__ __align__(1024) T slabs[kSlots][kSlab];
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
         const uint32_t stride_a = FORM == kMatrixGrad ? g.m : g.k, stride_b = FORM == kForward ? g.k : g.n;
-        const size_t   move_a = A_DEPTH ? kDepthStep : (size_t) kDepthStep * stride_a, move_b = B_DEPTH ? kDepthStep : (size_t) kDepthStep * stride_b;
-        const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void*) slabs + wave * 1024;
+        const size_t   move_a = A_DEPTH ? kStep<T> : (size_t) kStep<T> * stride_a, move_b = B_DEPTH ? kStep<T> : (size_t) kStep<T> * stride_b;
+        const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void*) slabs + wave * (64 * SlabA::kPiece);
+        constexpr uint32_t kSlabBytes = kSlab * sizeof(T);
 
         RowTiles       tiles{};
         const uint32_t m_tiles = (g.m + BM - 1) / BM;// kMatrixGrad: row tiles of an expert
         if (FORM != kMatrixGrad) tiles = row_tiles_of(BM, g.n_experts, g.n_places, g.offsets);
         const Patches  patches = patches_of(FORM == kMatrixGrad ? g.n_experts * m_tiles : tiles.total, col_tiles);
-        const uint32_t team = gridDim.x / 8, member = blockIdx.x / 8;// (the grid is a multiple of 8)
+        const uint32_t team = gridDim.x / 8;// (the grid is a multiple of 8)
 
         // the tile at hand
         const T *      A, *B;
         T*             C;
         uint32_t       rows, cols, depth, steps, whole;
         uint32_t       off_a[LOADS], off_b[LOADS];
-        // the XCD's tiles are numbered patch by patch; at >= its count: done
+        // the XCD's tiles are numbered patch by patch
         const uint32_t area = patches.width * patches.height;
-        uint32_t       at   = member;
+        uint32_t       at   = blockIdx.x / 8;
         auto           next = [&]() -> bool {
             for (;; at += team) {
                 const uint32_t p = at / area * 8 + blockIdx.x % 8, in = at % area;
@@ -365,17 +339,17 @@ namespace splahip {
                     B = static_cast<const T*>(g.b) + (size_t) begin * g.n + n0;
                     C = static_cast<T*>(g.c) + ((size_t) expert * g.m + m0) * g.n + n0;
                 } else {
-                    const RowTile t = row_tile(tiles, row, BM, g.n_experts, g.n_places, g.offsets);
+                    const RowTile  t = row_tile(tiles, row, BM, g.n_experts, g.n_places, g.offsets);
                     const uint32_t e = min(t.expert, g.n_experts - 1);
-                    rows            = t.rows;
-                    depth           = t.expert < g.n_experts ? g.k : 0u;
+                    rows             = t.rows;
+                    depth            = t.expert < g.n_experts ? g.k : 0u;
                     A = static_cast<const T*>(g.a) + (size_t) t.row0 * g.k;
                     B = static_cast<const T*>(g.b) + (FORM == kForward ? ((size_t) e * g.n + n0) * g.k : (size_t) e * g.n * g.k + n0);
                     C = static_cast<T*>(g.c) + (size_t) t.row0 * g.n + n0;
                 }
                 A = uniform(A), B = uniform(B), C = uniform(C);
                 rows = __builtin_amdgcn_readfirstlane(rows), depth = __builtin_amdgcn_readfirstlane(depth);
-                steps = (depth + kDepthStep - 1) / kDepthStep, whole = depth / kDepthStep;
+                steps = (depth + kStep<T> - 1) / kStep<T>, whole = depth / kStep<T>;
                 uint32_t sa = stride_a, sb = stride_b;// (opaque: what depends on them is made anew for each tile, not kept in registers)
                 asm volatile("" : "+s"(sa), "+s"(sb));
                 SlabA::offsets(sa, rows, off_a);
@@ -385,36 +359,52 @@ namespace splahip {
             }
         };
         auto slot_after = [](uint32_t slot, uint32_t n) { return slot + n >= kSlots ? slot + n - kSlots : slot + n; };
-        auto load_a = [&](uint32_t s, uint32_t slot, uint32_t i) { load_to_lds_at(A + s * move_a, off_a[i], lds0 + slot * (kSlab * 2) + i * (THREADS * 16)); };
-        auto load_b = [&](uint32_t s, uint32_t slot, uint32_t i) { load_to_lds_at(B + s * move_b, off_b[i], lds0 + slot * (kSlab * 2) + i * (THREADS * 16)); };
-        auto slab_a = [&](uint32_t s, uint32_t slot) {
-            if (s < whole) {
+        auto dst_of     = [&](uint32_t slot) { return lds0 + slot * kSlabBytes; };
+        auto slab_a     = [&](uint32_t s, uint32_t slot) {
+            if constexpr (LOAD != kElements) {
+                if (s < whole) {
 #pragma unroll
-                for (uint32_t i = 0; i < LOADS; ++i) load_a(s, slot, i);
-            } else if (s < steps)
-                last_slab<SlabA>(A + s * move_a, off_a, depth - s * kDepthStep, lds0 + slot * (kSlab * 2), THREADS * 16);
+                    for (uint32_t i = 0; i < LOADS; ++i) SlabA::load(A + s * move_a, off_a, i, dst_of(slot));
+                } else if (s < steps)
+                    SlabA::load_last(A + s * move_a, off_a, depth - s * kStep<T>, dst_of(slot));
+            }
         };
         auto slab_b = [&](uint32_t s, uint32_t slot) {
-            if (s < whole) {
+            if constexpr (LOAD != kElements) {
+                if (s < whole) {
 #pragma unroll
-                for (uint32_t i = 0; i < LOADS; ++i) load_b(s, slot, i);
-            } else if (s < steps)
-                last_slab<SlabB>(B + s * move_b, off_b, depth - s * kDepthStep, lds0 + slot * (kSlab * 2), THREADS * 16);
+                    for (uint32_t i = 0; i < LOADS; ++i) SlabB::load(B + s * move_b, off_b, i, dst_of(slot));
+                } else if (s < steps)
+                    SlabB::load_last(B + s * move_b, off_b, depth - s * kStep<T>, dst_of(slot));
+            }
         };
+        // kElements: a slab of each operand on its way
+        s16x8 ra[LOADS], rb[LOADS];
+        auto  fetch_a = [&](uint32_t s) { if (s < steps) SlabA::fetch(A + s * move_a, off_a, rows, min(kStep<T>, depth - s * kStep<T>), ra); };
+        auto  fetch_b = [&](uint32_t s) { if (s < steps) SlabB::fetch(B + s * move_b, off_b, cols, min(kStep<T>, depth - s * kStep<T>), rb); };
 
         if (!next()) return;
         slab_a(0, 0), slab_b(0, 1), slab_a(1, 2), slab_b(1, 3);
-        bool stored = false;// a whole tile's stores are among the loads under way
+        bool stored = false;// a whole tile's stores are among what is under way
         for (bool more = true; more;) {
             f32x16 acc[TM][TN] = {};
             slab_a(2, 4);
             if (steps) {
-                // the first two slabs: behind them three more, and a whole tile's stores
-                if (whole < 3) loads_arrived<0>();
-                else if (stored)
-                    loads_arrived<3 * LOADS + kStores>();
-                else
-                    loads_arrived<3 * LOADS>();
+                if constexpr (LOAD == kElements) {
+                    fetch_a(0), fetch_b(0);
+                    SlabA::put(ra, slabs[0]), SlabB::put(rb, slabs[1]);
+                    fetch_a(1);
+                    SlabA::put(ra, slabs[2]);
+                    fetch_b(1), fetch_a(2);
+                } else {
+                    // the first two slabs: behind them three more, and a whole tile's stores
+                    constexpr uint32_t kBehind = 3 * LOADS + kStores < 64 ? 3 * LOADS + kStores : 3 * LOADS;
+                    if (whole < 3) loads_arrived<0>();
+                    else if (stored)
+                        loads_arrived<kBehind>();
+                    else
+                        loads_arrived<3 * LOADS>();
+                }
                 __syncthreads();
                 s16x8 fa[2][TM], fb[2][TN];
 #pragma unroll
@@ -423,19 +413,22 @@ namespace splahip {
                 for (uint32_t i = 0; i < TM; ++i) fa[0][i] = operand<T, BM, A_DEPTH>(slabs[0], wm + i * 32, 0);
                 // quarter q's matrix instructions; the next quarter's operands are read meanwhile, and with `load` the loads of B's slab ls and A's next one issued
                 auto quarter = [&](auto q_, auto load_, const T* as, const T* bs, uint32_t ls, uint32_t slot) {
-                    constexpr uint32_t q = decltype(q_)::value, cur = q & 1u, k0 = (q + 1) % 4 * 16;
-                    constexpr bool     load = decltype(load_)::value;
+                    constexpr uint32_t q = decltype(q_)::value, cur = q & 1u, k0 = (q + 1) % 4 * kQuarter;
+                    constexpr bool     load = decltype(load_)::value && LOAD != kElements;
 #pragma unroll
                     for (uint32_t x = 0; x < kMul; ++x) {
-                        if (x < TN) fb[cur ^ 1][x] = operand<T, BN, B_DEPTH>(bs, wn + x * 32, k0);
-                        else if (x < kReads)
-                            fa[cur ^ 1][x - TN] = operand<T, BM, A_DEPTH>(as, wm + (x - TN) * 32, k0);
-                        if (load)
+#pragma unroll
+                        for (uint32_t r = x * kReadsPer; r < (x + 1) * kReadsPer && r < kReads; ++r) {
+                            if (r < TN) fb[cur ^ 1][r] = operand<T, BN, B_DEPTH>(bs, wn + r * 32, k0);
+                            else
+                                fa[cur ^ 1][r - TN] = operand<T, BM, A_DEPTH>(as, wm + (r - TN) * 32, k0);
+                        }
+                        if constexpr (load)
 #pragma unroll
                             for (uint32_t l = x * 2 * LOADS / kMul; l < (x + 1) * 2 * LOADS / kMul; ++l) {
-                                if (l < LOADS) load_b(ls, slot, l);
+                                if (l < LOADS) SlabB::load(B + ls * move_b, off_b, l, dst_of(slot));
                                 else
-                                    load_a(ls + 1, slot_after(slot, 1), l - LOADS);
+                                    SlabA::load(A + (ls + 1) * move_a, off_a, l - LOADS, dst_of(slot_after(slot, 1)));
                             }
                         acc[x / TN][x % TN] = matrix_step(fb[cur][x % TN], fa[cur][x / TN], acc[x / TN][x % TN], T{});
                         __builtin_amdgcn_sched_barrier(0);
@@ -450,17 +443,22 @@ namespace splahip {
                     quarter(integral_constant<uint32_t, 0>{}, no, as, bs, 0, 0);
                     quarter(integral_constant<uint32_t, 1>{}, no, as, bs, 0, 0);
                     quarter(integral_constant<uint32_t, 2>{}, no, as, bs, 0, 0);
-                    if (decltype(load_)::value) loads_arrived<LOADS>();
+                    if constexpr (LOAD == kElements) SlabB::put(rb, slabs[slot_after(slot, 3)]), SlabA::put(ra, slabs[slot_after(slot, 4)]);
+                    else if (decltype(load_)::value)
+                        loads_arrived<LOADS>();
                     else
                         loads_arrived<0>();
                     __syncthreads();
                     // B's slab s + 2 goes where A's s was, A's s + 3 where B's s was
-                    if (!decltype(load_)::value) slab_b(s + 2, slot), slab_a(s + 3, slot_after(slot, 1));
+                    if constexpr (LOAD == kElements) fetch_b(s + 2), fetch_a(s + 3);
+                    else if (!decltype(load_)::value)
+                        slab_b(s + 2, slot), slab_a(s + 3, slot_after(slot, 1));
                     quarter(integral_constant<uint32_t, 3>{}, load_, slabs[slot_after(slot, 2)], slabs[slot_after(slot, 3)], s + 2, slot);
                     slot = slot_after(slot, 2);
                 };
                 uint32_t s = 0;
-                for (; s + 3 < whole; ++s) step(yes, s);
+                if constexpr (LOAD != kElements)
+                    for (; s + 3 < whole; ++s) step(yes, s);
                 for (; s < steps; ++s) step(no, s);
                 __syncthreads();// nothing reads a slab any more
             }
@@ -471,37 +469,56 @@ namespace splahip {
             more = next();
             if (more) slab_a(0, 0), slab_b(0, 1), slab_a(1, 2), slab_b(1, 3);
             stored = out_rows == BM && out_cols == BN;
-            // A lane holds four neighbouring columns (8 bytes) of a row, its neighbours hold other rows.  Every wavefront turns its part in the fifth slab, 32 rows at a time, and stores
-            // rows of BN / WN columns.
-            T*   turn = slabs[4] + wave * (32 * kCols);
-            auto swz  = [](uint32_t m) { return (m / (16 / kRowUnits)) % kRowUnits; };
+            // A lane holds four neighbouring columns of a row, its neighbours hold other rows.
+            auto quad = [&](uint32_t i, uint32_t j, uint32_t v) {
+                typedef T four __attribute__((ext_vector_type(4)));
+                four      c;
 #pragma unroll
-            for (uint32_t i = 0; i < TM; ++i) {
-                const uint32_t m = lane & 31u;
+                for (uint32_t q = 0; q < 4; ++q) c[q] = (T) acc[i][j][v + q];
+                return c;
+            };
+            if constexpr (kTurns) {
+                // every wavefront turns its part in LDS and stores lines
+                T*   turn = slabs[4] + wave * (32 * kTurnCols);
+                auto swz  = [](uint32_t m) { return (m / (16 / kRowUnits)) % kRowUnits; };
 #pragma unroll
-                for (uint32_t j = 0; j < TN; ++j)
+                for (uint32_t i = 0; i < TM; ++i)
 #pragma unroll
-                    for (uint32_t v = 0; v < 16; v += 4) {
-                        typedef T four __attribute__((ext_vector_type(4)));
-                        four      c;
+                    for (uint32_t j0 = 0; j0 < TN; j0 += kTurn) {
+                        const uint32_t m = lane & 31u;
 #pragma unroll
-                        for (uint32_t q = 0; q < 4; ++q) c[q] = (T) acc[i][j][v + q];
-                        const uint32_t unit = j * 4 + v / 4;
-                        *reinterpret_cast<four*>(turn + m * kCols + ((unit ^ swz(m)) * 8 + (lane >> 5) * 4)) = c;
+                        for (uint32_t j = 0; j < kTurn; ++j)
+#pragma unroll
+                            for (uint32_t v = 0; v < 16; v += 4) {
+                                const auto     c = quad(i, j0 + j, v);
+                                const uint32_t n = j * 32 + v * 2 + (lane >> 5) * 4;
+                                __builtin_memcpy(__builtin_assume_aligned(turn + m * kTurnCols + (((n / kUnit<T>) ^ swz(m)) * kUnit<T> + n % kUnit<T>), 4 * sizeof(T)), &c, sizeof c);
+                            }
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                        for (uint32_t x = 0; x < 32 * kRowUnits / 64; ++x) {
+                            const uint32_t u = x * 64 + lane, row = u / kRowUnits, unit = u % kRowUnits;
+                            s16x8          c;
+                            __builtin_memcpy(&c, __builtin_assume_aligned(turn + row * kTurnCols + (unit ^ swz(row)) * kUnit<T>, 16), 16);
+                            const uint32_t gm = wm + i * 32 + row, gn = wn + j0 * 32 + unit * kUnit<T>;
+                            if (gm < out_rows && gn < out_cols) store_part(out + (size_t) gm * ldc + gn, out_cols - gn, c);
+                        }
+                        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                        __builtin_amdgcn_wave_barrier();
                     }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                if (more) __syncthreads();// the fifth slab is free again
+            } else {
 #pragma unroll
-                for (uint32_t x = 0; x < 32 * kRowUnits / 64; ++x) {
-                    const uint32_t u = x * 64 + lane, row = u / kRowUnits, unit = u % kRowUnits;
-                    const s16x8    c = *reinterpret_cast<const s16x8*>(turn + row * kCols + ((unit ^ swz(row)) * 8));
-                    const uint32_t gm = wm + i * 32 + row, gn = wn + unit * 8;
-                    if (gm < out_rows && gn < out_cols) *reinterpret_cast<s16x8*>(out + (size_t) gm * ldc + gn) = c;// (columns come in eights)
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                for (uint32_t i = 0; i < TM; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < TN; ++j)
+#pragma unroll
+                        for (uint32_t v = 0; v < 16; v += 4) {
+                            const uint32_t gm = wm + i * 32 + (lane & 31u), gn = wn + j * 32 + v * 2 + (lane >> 5) * 4;
+                            if (gm < out_rows && gn < out_cols) store_part(out + (size_t) gm * ldc + gn, out_cols - gn, __builtin_bit_cast(s16x8, quad(i, j, v)));
+                        }
             }
-            if (more) __syncthreads();// the fifth slab is free again
         }
     }
 
@@ -509,42 +526,41 @@ namespace splahip {
         SPLAHIP_REQUIRE(panel_type_valid(panel_type), "panel type");
         SPLAHIP_REQUIRE(n_experts >= 1 && n_experts <= 2048, "experts: 1 .. 2048");
         SPLAHIP_REQUIRE(n_places < (1u << 31), "rows: below 2^31");
-        SPLAHIP_REQUIRE(n_in >= 1 && n_out >= 1 && n_in < (1u << 24) && n_out < (1u << 24), "matrix sizes: 1 .. 2^24 - 1");
+        SPLAHIP_REQUIRE(n_in >= 1 && n_out >= 1 && n_in < (1u << 21) && n_out < (1u << 21), "matrix sizes: 1 .. 2^21 - 1");
         return SPLAHIP_OK;
     }
 
-    template<typename T, Form FORM, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC>
-    static int launch_tiles(const GeneralArgs& g, hipStream_t s) {
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC>
+    static int launch_tiles(const ProductArgs& g, hipStream_t s) {
         const uint64_t col_tiles = (g.n + BM - 1) / BM;
         const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + BM - 1) / BM) : row_tiles_bound(g.n_places, g.n_experts, BM);
         SPLAHIP_REQUIRE(col_tiles * row_tiles < (1ull << 31), "too many tiles for one launch");
         constexpr uint32_t kResident = 256 * (OCC * 4 / (WM * WN));// workgroups the card holds at once
-        product_tile_kernel<T, FORM, BM, WM, WN, OCC><<<kResident, WM * WN * 64, 0, s>>>(g, (uint32_t) col_tiles);
+        product_kernel<T, FORM, LOAD, BM, WM, WN, OCC><<<kResident, WM * WN * 64, 0, s>>>(g, (uint32_t) col_tiles);
+        SPLAHIP_TRY(hipGetLastError());
         return SPLAHIP_OK;
     }
 
-    template<Form FORM>
-    static int launch_product(int panel_type, const GeneralArgs& g, hipStream_t s) {
-        const bool units = g.n < (1u << 22) && g.k < (1u << 22) && g.m < (1u << 22) && ((uintptr_t) g.a % 16 == 0) && ((uintptr_t) g.b % 16 == 0) && ((uintptr_t) g.c % 16 == 0) && g.n % 8 == 0 && g.k % 8 == 0 && g.m % 8 == 0;
-        int        st    = SPLAHIP_OK;
-        if (panel_type != SPLAHIP_PANEL_FLOAT && units) {
-            const uint64_t tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + 255) / 256) * ((g.n + 255) / 256) : (uint64_t) (g.n_places / 256 + 1) * ((g.n + 255) / 256);
-            const bool     large = tiles >= 200;
-            if (panel_type == SPLAHIP_PANEL_HALF) st = large ? launch_tiles<fp16_t, FORM, 256, 2, 4, 2>(g, s) : launch_tiles<fp16_t, FORM, 128, 2, 2, 2>(g, s);
-            else
-                st = large ? launch_tiles<bf16_t, FORM, 256, 2, 4, 2>(g, s) : launch_tiles<bf16_t, FORM, 128, 2, 2, 2>(g, s);
-            if (st) return st;
-            SPLAHIP_TRY(hipGetLastError());
-            return SPLAHIP_OK;
+    template<Form FORM, typename T>
+    static int launch_of_type(const ProductArgs& g, hipStream_t s) {
+        const uint32_t u       = kUnit<T>;
+        const bool     aligned = ((uintptr_t) g.a % 16 == 0) && ((uintptr_t) g.b % 16 == 0) && ((uintptr_t) g.c % 16 == 0) && g.n % u == 0 && g.k % u == 0 && g.m % u == 0;
+        auto tiles = [&](uint64_t bm) { return (FORM == kMatrixGrad ? g.n_experts * ((g.m + bm - 1) / bm) : g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
+        if constexpr (sizeof(T) == 4) {
+            const bool large = tiles(128) >= 400;
+            if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);
+            return large ? launch_tiles<T, FORM, kWords, 128, 2, 2, 2>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
+        } else {
+            if (!aligned) return launch_tiles<T, FORM, kElements, 128, 2, 2, 2>(g, s);
+            return tiles(256) >= 200 ? launch_tiles<T, FORM, kUnits, 256, 2, 4, 2>(g, s) : launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s);
         }
-        const uint64_t col_tiles = (g.n + 63) / 64;
-        const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + 63) / 64) : row_tiles_bound(g.n_places, g.n_experts, 64);
-        SPLAHIP_REQUIRE(col_tiles * row_tiles < (1ull << 31), "too many tiles for one launch");
-        panel_dispatch(panel_type, [&](auto zero) {
-            product_general_kernel<decltype(zero), FORM><<<(uint32_t) (col_tiles * row_tiles), 256, 0, s>>>(g, (uint32_t) col_tiles);
-        });
-        SPLAHIP_TRY(hipGetLastError());
-        return SPLAHIP_OK;
+    }
+
+    template<Form FORM>
+    static int launch_product(int panel_type, const ProductArgs& g, hipStream_t s) {
+        int st = SPLAHIP_OK;
+        panel_dispatch(panel_type, [&](auto zero) { st = launch_of_type<FORM, decltype(zero)>(g, s); });
+        return st;
     }
 
 }// namespace splahip
@@ -557,7 +573,7 @@ extern "C" int splahip_expert_product(int panel_type, uint32_t n_places, uint32_
     if (n_places == 0) return SPLAHIP_OK;
     SPLAHIP_REQUIRE(d_offsets && d_x && d_w && d_y, "null array");
     if (int st = ensure_device()) return st;
-    return launch_product<kForward>(panel_type, GeneralArgs{d_x, d_w, d_y, n_places, n_experts, 0, n_out, n_in, d_offsets}, as_stream(stream));
+    return launch_product<kForward>(panel_type, ProductArgs{d_x, d_w, d_y, n_places, n_experts, 0, n_out, n_in, d_offsets}, as_stream(stream));
 }
 
 extern "C" int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets,
@@ -566,7 +582,7 @@ extern "C" int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint
     if (n_places == 0) return SPLAHIP_OK;
     SPLAHIP_REQUIRE(d_offsets && d_dy && d_w && d_dx, "null array");
     if (int st = ensure_device()) return st;
-    return launch_product<kRowGrad>(panel_type, GeneralArgs{d_dy, d_w, d_dx, n_places, n_experts, 0, n_in, n_out, d_offsets}, as_stream(stream));
+    return launch_product<kRowGrad>(panel_type, ProductArgs{d_dy, d_w, d_dx, n_places, n_experts, 0, n_in, n_out, d_offsets}, as_stream(stream));
 }
 
 extern "C" int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets,
@@ -574,5 +590,5 @@ extern "C" int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint
     if (int st = check_product(panel_type, n_places, n_experts, n_in, n_out)) return st;
     SPLAHIP_REQUIRE(d_offsets && d_dw && (n_places == 0 || (d_dy && d_x)), "null array");
     if (int st = ensure_device()) return st;
-    return launch_product<kMatrixGrad>(panel_type, GeneralArgs{d_dy, d_x, d_dw, n_places, n_experts, n_out, n_in, 0, d_offsets}, as_stream(stream));
+    return launch_product<kMatrixGrad>(panel_type, ProductArgs{d_dy, d_x, d_dw, n_places, n_experts, n_out, n_in, 0, d_offsets}, as_stream(stream));
 }
