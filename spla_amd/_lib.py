@@ -134,7 +134,7 @@ _SIGNATURES = {
     "splahip_expert_product": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
     "splahip_expert_product_dx": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
     "splahip_expert_product_dw": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
-    "splahip_global_norm_workspace": (C.c_size_t, [C.c_uint32, C.POINTER(C.c_uint64)]),
+    "splahip_global_norm_workspace": (C.c_size_t, [C.c_uint32, _vp]),
     "splahip_global_norm": (C.c_int, [C.c_uint32, _vp, _vp, _vp, _vp, C.c_size_t, _vp, _vp]),
     "splahip_clip_global_norm": (C.c_int, [C.c_uint32, _vp, _vp, _vp, _vp, C.c_float, C.c_int, _vp, C.c_size_t, _vp, _vp]),
 }

@@ -522,6 +522,107 @@ namespace splahip {
         }
     }
 
+    // ---- few rows per expert -----------------------------------------------------------------------------------------------------------------------------
+    // Serving: every matrix is read for a few rows, the time is that of reading them.  A workgroup computes all rows of an expert x 16 NF columns, 32 at a time (for more, its
+    // part of the matrix is read again, from the cache); its four wavefronts take the depth in turns of 128 bytes, so that a matrix row is read in runs of
+    // 512, and go from memory to the matrix instruction without LDS: lane l holds row l % 16, 16 bytes of k from unit l / 16.  The wavefronts' sums are joined in LDS in
+    // a fixed order.  Many small workgroups instead of a few that stay: what counts is bytes under way.
+    __device__ __forceinline__ f32x4 matrix_step16(s16x8 a, s16x8 b, f32x4 c, bf16_t) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x4 matrix_step16(s16x8 a, s16x8 b, f32x4 c, fp16_t) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
+    }
+    __device__ __forceinline__ f32x4 matrix_step16(s16x8 a, s16x8 b, f32x4 c, float) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    }
+
+    constexpr uint32_t kZeroBlocks = 64;// workgroups for the rows behind the last entry
+
+    template<typename T, uint32_t NF>
+    __global__ __launch_bounds__(256) void product_few_rows_kernel(const ProductArgs g, uint32_t col_tiles) {
+        constexpr uint32_t MF = 2, U = kUnit<T>, CHUNK = 8 * U, AHEAD = 2;// chunks of a wavefront under way
+        __shared__ f32x4   part[4][NF * MF][64];
+        const uint32_t     lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        const uint32_t     expert = blockIdx.x / col_tiles;
+        typedef T          four __attribute__((ext_vector_type(4)));
+        if (expert >= g.n_experts) {
+            const uint64_t end = (uint64_t) g.n_places * (g.n / 4), step = (uint64_t) (gridDim.x - g.n_experts * col_tiles) * 256;
+            for (uint64_t i = (uint64_t) bounded(g.offsets, g.n_experts, g.n_experts, g.n_places) * (g.n / 4) + (blockIdx.x - g.n_experts * col_tiles) * 256 + threadIdx.x; i < end; i += step)
+                reinterpret_cast<four*>(g.c)[i] = four{};
+            return;
+        }
+        const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
+        const uint32_t n0 = blockIdx.x % col_tiles * (16 * NF), depth = g.k;
+        const T*       w[NF];
+#pragma unroll
+        for (uint32_t j = 0; j < NF; ++j)
+            w[j] = static_cast<const T*>(g.b) + ((size_t) expert * g.n + min(n0 + j * 16 + (lane & 15u), g.n - 1)) * g.k + (lane >> 4) * U;
+        for (uint32_t row0 = begin; row0 < end; row0 += 16 * MF) {
+            const uint32_t rows = end - row0;
+            const T*       x[MF];
+#pragma unroll
+            for (uint32_t i = 0; i < MF; ++i) x[i] = static_cast<const T*>(g.a) + (size_t) (row0 + min(i * 16 + (lane & 15u), rows - 1)) * g.k + (lane >> 4) * U;
+            f32x4 acc[MF][NF] = {};
+            for (uint32_t k0 = wave * CHUNK; k0 < depth; k0 += 4 * CHUNK * AHEAD) {
+                s16x8 a[AHEAD][2][NF], b[AHEAD][2][MF];
+#pragma unroll
+                for (uint32_t c = 0; c < AHEAD; ++c) {
+#pragma unroll
+                    for (uint32_t j = 0; j < NF; ++j)
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const uint32_t k = k0 + c * 4 * CHUNK + h * 4 * U;
+                            a[c][h][j]       = k + (lane >> 4) * U < depth ? *reinterpret_cast<const s16x8*>(w[j] + k) : s16x8{};// (the depth comes in whole units)
+                        }
+#pragma unroll
+                    for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const uint32_t k = k0 + c * 4 * CHUNK + h * 4 * U;
+                            b[c][h][i]       = k + (lane >> 4) * U < depth ? *reinterpret_cast<const s16x8*>(x[i] + k) : s16x8{};
+                        }
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < AHEAD; ++c)
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                        for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+                            for (uint32_t j = 0; j < NF; ++j) acc[i][j] = matrix_step16(a[c][h][j], b[c][h][i], acc[i][j], T{});
+            }
+            __syncthreads();// (the last rows' sums have been read)
+#pragma unroll
+            for (uint32_t i = 0; i < MF; ++i)
+#pragma unroll
+                for (uint32_t j = 0; j < NF; ++j) part[wave][i * NF + j][lane] = acc[i][j];
+            __syncthreads();
+            for (uint32_t f = wave; f < MF * NF; f += 4) {
+                const f32x4    sum = (part[0][f][lane] + part[1][f][lane]) + (part[2][f][lane] + part[3][f][lane]);
+                const uint32_t m = f / NF * 16 + (lane & 15u), n = n0 + f % NF * 16 + (lane >> 4) * 4;
+                if (m < rows && n < g.n) {// (columns come in fours)
+                    four c;
+#pragma unroll
+                    for (uint32_t q = 0; q < 4; ++q) c[q] = (T) sum[q];
+                    *reinterpret_cast<four*>(static_cast<T*>(g.c) + (size_t) (row0 + m) * g.n + n) = c;
+                }
+            }
+        }
+    }
+
+    template<typename T, uint32_t NF>
+    static int launch_few_rows(const ProductArgs& g, hipStream_t s) {
+        const uint64_t col_tiles = (g.n + 16 * NF - 1) / (16 * NF), blocks = g.n_experts * col_tiles + kZeroBlocks;
+        SPLAHIP_REQUIRE(blocks < (1ull << 31), "too many tiles for one launch");
+        product_few_rows_kernel<T, NF><<<(uint32_t) blocks, 256, 0, s>>>(g, (uint32_t) col_tiles);
+        SPLAHIP_TRY(hipGetLastError());
+        return SPLAHIP_OK;
+    }
+
     static int check_product(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out) {
         SPLAHIP_REQUIRE(panel_type_valid(panel_type), "panel type");
         SPLAHIP_REQUIRE(n_experts >= 1 && n_experts <= 2048, "experts: 1 .. 2048");
@@ -546,6 +647,9 @@ namespace splahip {
         const uint32_t u       = kUnit<T>;
         const bool     aligned = ((uintptr_t) g.a % 16 == 0) && ((uintptr_t) g.b % 16 == 0) && ((uintptr_t) g.c % 16 == 0) && g.n % u == 0 && g.k % u == 0 && g.m % u == 0;
         auto tiles = [&](uint64_t bm) { return (FORM == kMatrixGrad ? g.n_experts * ((g.m + bm - 1) / bm) : g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
+        if constexpr (FORM == kForward)
+            if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts)
+                return min(g.n_places, g.n_experts) * (uint64_t) (g.n / 64) >= 1024 ? launch_few_rows<T, 4>(g, s) : launch_few_rows<T, 2>(g, s);
         if constexpr (sizeof(T) == 4) {
             const bool large = tiles(128) >= 400;
             if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);

@@ -85,6 +85,26 @@ namespace splahip {
         if (threadIdx.x == 0) totals[blockIdx.x] = base;
     }
 
+    // a wavefront's entries, 64 at a time from `first`: mine[e] (LDS) = where its next entry of e goes
+    __device__ __forceinline__ void place_wave(uint32_t first, uint32_t steps, uint32_t n_entries, uint32_t n_experts, uint32_t bits, const int32_t* __restrict__ experts,
+                                               int32_t* __restrict__ order, int32_t* __restrict__ place, uint32_t* mine) {
+        const uint32_t lane = threadIdx.x & 63u;
+        for (uint32_t s = 0; s < steps; ++s) {// (the wavefront's own words only: its LDS accesses stay in program order)
+            const uint32_t i     = first + s * 64 + lane;
+            const uint32_t e     = i < n_entries ? (uint32_t) experts[i] : ~0u;
+            const bool     valid = e < n_experts;
+            const uint64_t alike = lanes_alike(e, valid, bits);
+            const uint32_t below = __popcll(alike & ((1ull << lane) - 1ull));
+            uint32_t       p     = 0;
+            if (valid) p = *(volatile uint32_t*) &mine[e] + below;
+            if (i < n_entries) place[i] = valid ? (int32_t) p : -1;
+            if (valid) {
+                order[p] = (int32_t) i;
+                if (below == 0) *(volatile uint32_t*) &mine[e] = p + (uint32_t) __popcll(alike);
+            }
+        }
+    }
+
     // positions of the tile's entries; base[e] (LDS) = where the tile's first entry of e goes.  `waves` x n_experts words of LDS behind it.
     __device__ __forceinline__ void place_tile(uint32_t tile, uint32_t n_entries, uint32_t n_experts, uint32_t bits, const int32_t* __restrict__ experts,
                                                int32_t* __restrict__ order, int32_t* __restrict__ place, const uint32_t* base, uint32_t* wave_count, uint32_t n_waves,
@@ -110,20 +130,7 @@ namespace splahip {
             }
         }
         __syncthreads();
-        for (uint32_t s = 0; s < steps; ++s) {// (the wavefront's own words only: its LDS accesses stay in program order)
-            const uint32_t i     = first + s * 64 + lane;
-            const uint32_t e     = i < n_entries ? (uint32_t) experts[i] : ~0u;
-            const bool     valid = e < n_experts;
-            const uint64_t alike = lanes_alike(e, valid, bits);
-            const uint32_t below = __popcll(alike & ((1ull << lane) - 1ull));
-            uint32_t       p     = 0;
-            if (valid) p = *(volatile uint32_t*) &mine[e] + below;
-            if (i < n_entries) place[i] = valid ? (int32_t) p : -1;
-            if (valid) {
-                order[p] = (int32_t) i;
-                if (below == 0) *(volatile uint32_t*) &mine[e] = p + (uint32_t) __popcll(alike);
-            }
-        }
+        place_wave(first, steps, n_entries, n_experts, bits, experts, order, place, mine);
     }
 
     __global__ __launch_bounds__(256) void route_place_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t n_tiles, uint32_t bits, const int32_t* __restrict__ experts,
@@ -150,6 +157,42 @@ namespace splahip {
         }
         __syncthreads();
         place_tile(blockIdx.x, n_entries, n_experts, bits, experts, order, place, base, lds + n_experts, kSortWaves, kSortSteps);
+    }
+
+    // The whole sort in one workgroup of 16 wavefronts: a wavefront counts and places a contiguous part of the entries.
+    constexpr uint32_t kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64, kSmallEntries = 8192, kSmallExperts = 512;
+
+    __global__ __launch_bounds__(1024) void route_sort_small_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t bits, const int32_t* __restrict__ experts,
+                                                                    uint32_t* __restrict__ offsets, int32_t* __restrict__ order, int32_t* __restrict__ place) {
+        extern __shared__ uint32_t wave_count[];// kSmallWaves x n_experts
+        const uint32_t             lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+        const uint32_t             steps = (n_entries + kSmallThreads - 1) / kSmallThreads, first = wave * steps * 64;
+        for (uint32_t i = threadIdx.x; i < kSmallWaves * n_experts; i += kSmallThreads) wave_count[i] = 0;
+        __syncthreads();
+        for (uint32_t s = 0; s < steps; ++s) {
+            const uint32_t i = first + s * 64 + lane;
+            const uint32_t e = i < n_entries ? (uint32_t) experts[i] : ~0u;
+            if (e < n_experts) atomicAdd(&wave_count[wave * n_experts + e], 1u);
+        }
+        __syncthreads();
+        uint32_t mine = 0;// (n_experts <= kSmallThreads: a thread each)
+        if (threadIdx.x < n_experts)
+            for (uint32_t w = 0; w < kSmallWaves; ++w) mine += wave_count[w * n_experts + threadIdx.x];
+        uint32_t       all;
+        const uint32_t base = block_exclusive<kSmallThreads>(mine, &all);
+        if (threadIdx.x < n_experts) {
+            offsets[threadIdx.x] = base;
+            uint32_t at          = base;
+            for (uint32_t w = 0; w < kSmallWaves; ++w) {
+                const uint32_t c                              = wave_count[w * n_experts + threadIdx.x];
+                wave_count[w * n_experts + threadIdx.x] = at;
+                at += c;
+            }
+        }
+        if (threadIdx.x == 0) offsets[n_experts] = all;
+        for (uint32_t p = all + threadIdx.x; p < n_entries; p += kSmallThreads) order[p] = -1;
+        __syncthreads();
+        place_wave(first, steps, n_entries, n_experts, bits, experts, order, place, wave_count + wave * n_experts);
     }
 
     // ---- panels ----------------------------------------------------------------------------------------------------------------------------------------
@@ -287,7 +330,10 @@ namespace splahip {
 
 using namespace splahip;
 
+static bool sorts_small(uint64_t n_entries, uint32_t n_experts) { return n_entries <= kSmallEntries && n_experts <= kSmallExperts; }
+
 extern "C" size_t splahip_route_sort_workspace(uint32_t n_rows, uint32_t per_row, uint32_t n_experts) {
+    if (sorts_small((uint64_t) n_rows * per_row, n_experts)) return 0;
     const size_t tiles = ((size_t) n_rows * per_row + kSortTile - 1) / kSortTile;
     return ((size_t) n_experts * tiles + n_experts) * 4;
 }
@@ -298,11 +344,17 @@ extern "C" int splahip_route_sort(uint32_t n_rows, uint32_t per_row, uint32_t n_
     const uint32_t n     = n_rows * per_row;
     const uint32_t tiles = (n + kSortTile - 1) / kSortTile;
     SPLAHIP_REQUIRE(d_offsets && (n == 0 || (d_experts && d_order && d_place)), "null array");
-    SPLAHIP_REQUIRE(workspace_bytes >= splahip_route_sort_workspace(n_rows, per_row, n_experts) && d_workspace, "workspace too small");
+    const size_t need = splahip_route_sort_workspace(n_rows, per_row, n_experts);
+    SPLAHIP_REQUIRE(workspace_bytes >= need && (need == 0 || d_workspace), "workspace too small");
     if (int st = ensure_device()) return st;
     hipStream_t s    = as_stream(stream);
     uint32_t    bits = 0;
     while ((1u << bits) < n_experts) ++bits;
+    if (sorts_small(n, n_experts)) {
+        route_sort_small_kernel<<<1, kSmallThreads, n_experts * 4 * kSmallWaves, s>>>(n, n_experts, bits, d_experts, d_offsets, d_order, d_place);
+        SPLAHIP_TRY(hipGetLastError());
+        return SPLAHIP_OK;
+    }
     uint32_t* counts = static_cast<uint32_t*>(d_workspace);
     uint32_t* totals = counts + (size_t) n_experts * tiles;
     if (tiles) route_count_kernel<<<tiles, kSortThreads, n_experts * 4, s>>>(n, n_experts, tiles, d_experts, counts);

@@ -7,6 +7,7 @@ for uint32 words where torch has no unsigned dtype.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import torch
 
@@ -255,32 +256,36 @@ def mxm(t, a_rows, b_cols, A, B, op_mult, op_add, init, block_products=0, adopt=
 _PANEL_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-class _OnDevice:
-    """the device of a call's tensors made current for its launches"""
+_entries = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Python stream object around it (a fifth of a small call's time)
 
-    def __init__(self, device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(device, name, *args):
+    """call an entry point of the panel operators on the current stream of `device` (they read no environment knobs)"""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        raise _lib.SplaHipError(status, _lib.load().splahip_last_error().decode(errors="replace"))
 
 
 def _checked(name, t, dtype, shape, device=None):
     """t is a contiguous tensor on the GPU of this type, shape and device, else ValueError; returns its address"""
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.is_cuda and (device is None or t.device == device) and t.is_contiguous():
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: a tensor expected, not {type(t).__name__}")
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} expected, not {t.dtype} of {tuple(t.shape)}")
     if not t.is_cuda or (device is not None and t.device != device):
         raise ValueError(f"{name}: a tensor on {device or 'the GPU'} expected, not on {t.device}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: a contiguous tensor expected, not one of strides {t.stride()}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: a contiguous tensor expected, not one of strides {t.stride()}")
 
 
 def _panel_type(name, t):
@@ -295,10 +300,6 @@ def _width(name, t, rows):
     return t.shape[1]
 
 
-def _stream_of(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 class RoutePlan:
     """The entries of a routing matrix (n_rows tokens x n_experts, per_row entries a row) sorted by expert (route_sort).
 
@@ -307,23 +308,21 @@ class RoutePlan:
     place    int32 [n_rows, per_row]   the place of each entry, -1 for no entry
     """
 
-    __slots__ = ("offsets", "order", "place", "n_rows", "per_row", "n_experts")
+    __slots__ = ("offsets", "order", "place", "n_rows", "per_row", "n_places", "n_experts", "device")
 
     def __init__(self, offsets: torch.Tensor, order: torch.Tensor, place: torch.Tensor):
-        self.offsets, self.order, self.place = offsets, order, place
-        self.n_rows, self.per_row = place.shape
-        self.n_experts = offsets.numel() - 1
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or not isinstance(place, torch.Tensor) or place.dim() != 2:
+            raise ValueError("a plan's offsets are an int32 tensor [n_experts + 1], its places one of [n_rows, per_row]")
+        self._set(offsets, order, place)
         _checked("offsets", offsets, torch.int32, (self.n_experts + 1,))
-        _checked("order", order, torch.int32, (self.n_rows * self.per_row,), offsets.device)
-        _checked("place", place, torch.int32, (self.n_rows, self.per_row), offsets.device)
+        _checked("order", order, torch.int32, (self.n_places,), self.device)
+        _checked("place", place, torch.int32, (self.n_rows, self.per_row), self.device)
 
-    @property
-    def n_places(self):
-        return self.n_rows * self.per_row
-
-    @property
-    def device(self):
-        return self.offsets.device
+    def _set(self, offsets, order, place):
+        self.offsets, self.order, self.place, self.device = offsets, order, place, offsets.device
+        self.n_rows, self.per_row = place.shape
+        self.n_places, self.n_experts = self.n_rows * self.per_row, offsets.shape[0] - 1
+        return self
 
 
 def route_sort(experts: torch.Tensor, n_experts: int) -> RoutePlan:
@@ -335,15 +334,14 @@ def route_sort(experts: torch.Tensor, n_experts: int) -> RoutePlan:
     n_experts, device = int(n_experts), experts.device
     if not 1 <= n_experts <= 2048 or per_row < 1 or n_rows * per_row >= 1 << 31:
         raise ValueError(f"route_sort serves 1 .. 2048 experts, at least one entry a row and fewer than 2^31 entries, not {n_experts}, {per_row}, {n_rows * per_row}")
-    with _OnDevice(device):
-        offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
-        order = torch.empty(n_rows * per_row, dtype=torch.int32, device=device)
-        place = torch.empty(n_rows, per_row, dtype=torch.int32, device=device)
-        n_bytes = _lib.call("splahip_route_sort_workspace", n_rows, per_row, n_experts)
-        work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
-        _lib.call("splahip_route_sort", n_rows, per_row, n_experts, src, offsets.data_ptr(), order.data_ptr(), place.data_ptr(), work.data_ptr(), n_bytes,
-                  _stream_of(device))
-    return RoutePlan(offsets, order, place)
+    offsets = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
+    order = torch.empty(n_rows * per_row, dtype=torch.int32, device=device)
+    place = torch.empty_like(experts)
+    n_bytes = _lib.load().splahip_route_sort_workspace(n_rows, per_row, n_experts)
+    work = torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
+    _launch(device, "splahip_route_sort", n_rows, per_row, n_experts, src, offsets.data_ptr(), order.data_ptr(), place.data_ptr(),
+            work.data_ptr() if n_bytes else None, n_bytes)
+    return RoutePlan.__new__(RoutePlan)._set(offsets, order, place)
 
 
 def _weights(plan, weights):
@@ -356,10 +354,8 @@ def route_rows(plan: RoutePlan, x: torch.Tensor, weights: torch.Tensor = None) -
     t = _panel_type("x", x)
     width = _width("x", x, plan.n_rows)
     src, w = _checked("x", x, x.dtype, (plan.n_rows, width), plan.device), _weights(plan, weights)
-    with _OnDevice(plan.device):
-        out = torch.empty(plan.n_places, width, dtype=x.dtype, device=plan.device)
-        _lib.call("splahip_route_rows", t, plan.n_rows, plan.per_row, plan.n_experts, width, plan.offsets.data_ptr(), plan.place.data_ptr(), w, src, out.data_ptr(),
-                  _stream_of(plan.device))
+    out = torch.empty(plan.n_places, width, dtype=x.dtype, device=plan.device)
+    _launch(plan.device, "splahip_route_rows", t, plan.n_rows, plan.per_row, plan.n_experts, width, plan.offsets.data_ptr(), plan.place.data_ptr(), w, src, out.data_ptr())
     return out
 
 
@@ -368,9 +364,8 @@ def route_back(plan: RoutePlan, y: torch.Tensor, weights: torch.Tensor = None) -
     t = _panel_type("y", y)
     width = _width("y", y, plan.n_places)
     src, w = _checked("y", y, y.dtype, (plan.n_places, width), plan.device), _weights(plan, weights)
-    with _OnDevice(plan.device):
-        out = torch.empty(plan.n_rows, width, dtype=y.dtype, device=plan.device)
-        _lib.call("splahip_route_back", t, plan.n_rows, plan.per_row, width, plan.place.data_ptr(), w, src, out.data_ptr(), _stream_of(plan.device))
+    out = torch.empty(plan.n_rows, width, dtype=y.dtype, device=plan.device)
+    _launch(plan.device, "splahip_route_back", t, plan.n_rows, plan.per_row, width, plan.place.data_ptr(), w, src, out.data_ptr())
     return out
 
 
@@ -381,11 +376,9 @@ def route_back_grad(plan: RoutePlan, y: torch.Tensor, weights: torch.Tensor, dou
     src = _checked("y", y, y.dtype, (plan.n_places, width), plan.device)
     w = _checked("weights", weights, torch.float32, (plan.n_rows, plan.per_row), plan.device)
     g = _checked("dout", dout, y.dtype, (plan.n_rows, width), plan.device)
-    with _OnDevice(plan.device):
-        dy = torch.empty(plan.n_places, width, dtype=y.dtype, device=plan.device)
-        dweights = torch.empty(plan.n_rows, plan.per_row, dtype=torch.float32, device=plan.device)
-        _lib.call("splahip_route_back_grad", t, plan.n_rows, plan.per_row, plan.n_experts, width, plan.offsets.data_ptr(), plan.place.data_ptr(), w, src, g,
-                  dy.data_ptr(), dweights.data_ptr(), _stream_of(plan.device))
+    dy, dweights = torch.empty_like(y), torch.empty_like(weights)
+    _launch(plan.device, "splahip_route_back_grad", t, plan.n_rows, plan.per_row, plan.n_experts, width, plan.offsets.data_ptr(), plan.place.data_ptr(), w, src, g,
+            dy.data_ptr(), dweights.data_ptr())
     return dy, dweights
 
 
@@ -401,9 +394,8 @@ def expert_product(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor) -> torch.T
     t, src_w = _panel_type("x", x), _matrices(plan, w, x.dtype)
     n_out, n_in = w.shape[1:]
     src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
-    with _OnDevice(plan.device):
-        y = torch.empty(plan.n_places, n_out, dtype=x.dtype, device=plan.device)
-        _lib.call("splahip_expert_product", t, plan.n_places, plan.n_experts, n_in, n_out, plan.offsets.data_ptr(), src, src_w, y.data_ptr(), _stream_of(plan.device))
+    y = torch.empty(plan.n_places, n_out, dtype=x.dtype, device=plan.device)
+    _launch(plan.device, "splahip_expert_product", t, plan.n_places, plan.n_experts, n_in, n_out, plan.offsets.data_ptr(), src, src_w, y.data_ptr())
     return y
 
 
@@ -415,27 +407,38 @@ def expert_product_grad(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor, dy: t
     src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
     src_dy = _checked("dy", dy, x.dtype, (plan.n_places, n_out), plan.device)
     dx = dw = None
-    with _OnDevice(plan.device):
-        args, offsets, stream = (t, plan.n_places, plan.n_experts, n_in, n_out), plan.offsets.data_ptr(), _stream_of(plan.device)
-        if need[0]:
-            dx = torch.empty_like(x)
-            _lib.call("splahip_expert_product_dx", *args, offsets, src_dy, src_w, dx.data_ptr(), stream)
-        if need[1]:
-            dw = torch.empty_like(w)
-            _lib.call("splahip_expert_product_dw", *args, offsets, src_dy, src, dw.data_ptr(), stream)
+    args, offsets = (t, plan.n_places, plan.n_experts, n_in, n_out), plan.offsets.data_ptr()
+    if need[0]:
+        dx = torch.empty_like(x)
+        _launch(plan.device, "splahip_expert_product_dx", *args, offsets, src_dy, src_w, dx.data_ptr())
+    if need[1]:
+        dw = torch.empty_like(w)
+        _launch(plan.device, "splahip_expert_product_dw", *args, offsets, src_dy, src, dw.data_ptr())
     return dx, dw
 
 
+class _Words:
+    """a list of numbers as an array that an entry point reads"""
+
+    __slots__ = ("words", "ptr")
+
+    def __init__(self, code, numbers):
+        self.words = array(code, numbers)
+        self.ptr = self.words.buffer_info()[0]
+
+
 def _arrays(name, tensors):
-    """address, length and type lists of the tensors, all on one device"""
-    n = len(tensors)
-    ptrs, lengths, types = (C.c_void_p * n)(), (C.c_uint64 * n)(), (C.c_int * n)()
-    device = None
-    for i, t in enumerate(tensors):
-        types[i] = _panel_type(f"{name}[{i}]", t)
-        device = t.device if device is None else device
-        ptrs[i], lengths[i] = _checked(f"{name}[{i}]", t, t.dtype, t.shape, device), t.numel()
-    return ptrs, lengths, types, device
+    """address, length and type arrays of the tensors, all on one device"""
+    try:
+        types = _Words("i", [_PANEL_TYPE[t.dtype] for t in tensors])
+        same = len({t.device for t in tensors}) == 1 and tensors[0].is_cuda and all([t.is_contiguous() for t in tensors])
+    except (AttributeError, KeyError, TypeError):
+        same = False
+    if not same:  # say which
+        for i, t in enumerate(tensors):
+            _panel_type(f"{name}[{i}]", t)
+            _checked(f"{name}[{i}]", t, t.dtype, t.shape, tensors[0].device)
+    return _Words("Q", [t.data_ptr() for t in tensors]), _Words("Q", [t.numel() for t in tensors]), types, tensors[0].device
 
 
 def global_norm(tensors) -> torch.Tensor:
@@ -445,11 +448,10 @@ def global_norm(tensors) -> torch.Tensor:
     if not tensors:
         raise ValueError("tensors: at least one expected")
     ptrs, lengths, types, device = _arrays("tensors", tensors)
-    with _OnDevice(device):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        n_bytes = _lib.call("splahip_global_norm_workspace", len(tensors), lengths)
-        work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
-        _lib.call("splahip_global_norm", len(tensors), ptrs, lengths, types, work.data_ptr(), n_bytes, norm.data_ptr(), _stream_of(device))
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    n_bytes = _lib.load().splahip_global_norm_workspace(len(tensors), lengths.ptr)
+    work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
+    _launch(device, "splahip_global_norm", len(tensors), ptrs.ptr, lengths.ptr, types.ptr, work.data_ptr(), n_bytes, norm.data_ptr())
     return norm
 
 
@@ -465,16 +467,17 @@ def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None)
         out = list(out)
         if len(out) != len(tensors):
             raise ValueError(f"out: {len(tensors)} tensors expected, not {len(out)}")
-        out_ptrs = (C.c_void_p * len(out))(*[_checked(f"out[{i}]", o, t.dtype, t.shape, device) for i, (o, t) in enumerate(zip(out, tensors))])
-    given = norm is not None
-    with _OnDevice(device):
-        if given:
-            _checked("norm", norm, torch.float32, (), device)
-            work, n_bytes = None, 0
-        else:
-            norm = torch.empty((), dtype=torch.float32, device=device)
-            n_bytes = _lib.call("splahip_global_norm_workspace", len(tensors), lengths)
-            work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
-        _lib.call("splahip_clip_global_norm", len(tensors), ptrs, out_ptrs, lengths, types, float(limit), 1 if given else 0, work.data_ptr() if work is not None else None,
-                  n_bytes, norm.data_ptr(), _stream_of(device))
+        out_ptrs, _, _, out_device = _arrays("out", out)
+        if out_device != device or [t.dtype for t in out] != [t.dtype for t in tensors] or [t.shape for t in out] != [t.shape for t in tensors]:
+            for i, (o, t) in enumerate(zip(out, tensors)):
+                _checked(f"out[{i}]", o, t.dtype, t.shape, device)
+    if norm is not None:
+        _checked("norm", norm, torch.float32, (), device)
+        work, n_bytes, given = None, 0, 1
+    else:
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        n_bytes, given = _lib.load().splahip_global_norm_workspace(len(tensors), lengths.ptr), 0
+        work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
+    _launch(device, "splahip_clip_global_norm", len(tensors), ptrs.ptr, out_ptrs.ptr, lengths.ptr, types.ptr, float(limit), given, work.data_ptr() if work is not None else None,
+            n_bytes, norm.data_ptr())
     return norm

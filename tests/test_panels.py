@@ -15,7 +15,7 @@ def _plan(rows=4, k=2, experts=3):
     plan.offsets = torch.zeros(experts + 1, dtype=torch.int32)
     plan.order = torch.zeros(rows * k, dtype=torch.int32)
     plan.place = torch.zeros(rows, k, dtype=torch.int32)
-    plan.n_rows, plan.per_row, plan.n_experts = rows, k, experts
+    plan.n_rows, plan.per_row, plan.n_places, plan.n_experts, plan.device = rows, k, rows * k, experts, plan.offsets.device
     return plan
 
 
@@ -73,7 +73,8 @@ def test_c_entries_refuse():
     _fails("splahip_route_sort", 4, 2, 2049, p, p, p, p, p, big, None)        # too many experts
     _fails("splahip_route_sort", 1 << 30, 2, 3, p, p, p, p, p, big, None)     # 2^31 entries
     _fails("splahip_route_sort", 4, 2, 3, None, p, p, p, p, big, None)        # null
-    _fails("splahip_route_sort", 4, 2, 3, p, p, p, p, p, 8, None)             # workspace
+    _fails("splahip_route_sort", 1 << 16, 2, 3, p, p, p, p, p, 8, None)       # workspace
+    _fails("splahip_route_sort", 1 << 16, 2, 3, p, p, p, p, None, big, None)  # no workspace
     _fails("splahip_route_rows", 3, 4, 2, 3, 8, p, p, None, p, p, None)       # panel type
     _fails("splahip_route_rows", 0, 4, 2, 3, 1 << 30, p, p, None, p, p, None)  # width
     _fails("splahip_route_back", 0, 4, 2, 8, p, None, None, p, None)          # null
@@ -82,7 +83,7 @@ def test_c_entries_refuse():
         _fails(name, 7, 8, 3, 4, 4, p, p, p, p, None)
         _fails(name, 0, 8, 0, 4, 4, p, p, p, p, None)
         _fails(name, 0, 8, 3, 0, 4, p, p, p, p, None)
-        _fails(name, 0, 8, 3, 4, 1 << 24, p, p, p, p, None)
+        _fails(name, 0, 8, 3, 4, 1 << 21, p, p, p, p, None)
         _fails(name, 0, 8, 3, 4, 4, None, p, p, p, None)
         _fails(name, 0, 1 << 31, 3, 4, 4, p, p, p, p, None)
 
@@ -107,7 +108,7 @@ def test_clip_refuses_overlaps_and_limits():
 
 
 def test_workspaces_cover_the_largest():
-    assert _lib.call("splahip_route_sort_workspace", 0, 2, 8) >= 32
+    assert _lib.call("splahip_route_sort_workspace", 1 << 16, 2, 8) >= 32
     assert _lib.call("splahip_route_sort_workspace", (1 << 31) // 8 - 1, 8, 128) >= ((1 << 31) - 8) // 2048 * 128 * 4
     assert _lib.call("splahip_global_norm_workspace", 0, (C.c_uint64 * 1)()) >= 8
     assert _lib.call("splahip_global_norm_workspace", 2, (C.c_uint64 * 2)(0, 1)) >= 16
