@@ -96,23 +96,31 @@ namespace splahip {
         return RowTile{(uint32_t) e, begin + skip, min(bm, rows - skip)};
     }
 
-    // The tiles go to the workgroups in patches of about 32 neighbouring ones (up to 8 columns wide): a patch to the 32 CUs of one XCD, whose L2 then holds what they share, the
-    // patches to the XCDs in turn.  Workgroup b runs in XCD b % 8 and takes one tile of each of the XCD's patches.
     template<typename P>
     __device__ __forceinline__ P* uniform(P* p) {// the same in every lane, as the compiler may not see
         const uint64_t v = (uint64_t) p;
         return (P*) (((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32)) << 32) | (uint32_t) __builtin_amdgcn_readfirstlane((uint32_t) v));
     }
 
-    struct Patches {
-        uint32_t row_tiles, col_tiles, wide, width, height, count;
+    // Tile number t of a grid of row_tiles x col_tiles: H row tiles side by side, column by column, so that neighbouring tiles share both operands' slabs.
+    struct TileAt {
+        uint32_t row, col;
     };
-    __device__ __forceinline__ Patches patches_of(uint32_t row_tiles, uint32_t col_tiles) {
-        Patches p{row_tiles, col_tiles, (col_tiles + 7) / 8, 0, 0, 0};
-        p.width  = (col_tiles + p.wide - 1) / p.wide;
-        p.height = 32 / p.width;
-        p.count  = p.wide * ((row_tiles + p.height - 1) / p.height);
-        return p;
+    template<uint32_t H>
+    __device__ __forceinline__ TileAt tile_at(uint32_t t, uint32_t row_tiles, uint32_t col_tiles) {
+        const uint32_t group = t / (H * col_tiles), in = t % (H * col_tiles), height = min(H, row_tiles - group * H);
+        return TileAt{group * H + in % height, in / height};
+    }
+
+    // rank -> expert with the most rows first, for up to 64 experts (the order is free); lane = expert
+    __device__ __forceinline__ uint32_t rank_by_rows(uint32_t rows, uint32_t n_experts) {
+        const uint32_t lane = threadIdx.x & 63u;
+        uint32_t       rank = 0;
+        for (uint32_t e = 0; e < n_experts; ++e) {
+            const uint32_t r = __builtin_amdgcn_readlane(rows, e);
+            rank += r > rows || (r == rows && e < lane);
+        }
+        return rank;
     }
 
     // C[m, n] = sum over k of A(m, k) B(n, k).  A result tile is a workgroup's; rows of A and B are the result's rows and columns.
@@ -274,11 +282,16 @@ namespace splahip {
     // instructions run from registers, the operands of the next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last
     // quarter: behind it every wavefront has read this step's two slabs, so the next two loads may overwrite them, and the next step's slabs have arrived (issued one
     // step ago, A's two steps ago).  The loads of the next tile's first slabs are under way while a tile's result is stored.
-    // 16 bytes of a result row, or as many of their elements as the row has left
-    template<typename T>
+    // 16 bytes of a result row, or as many of their elements as the row has left.  A large result passes the L2 by: it would push out the slabs that the workgroups share
+    // (all of them store at about the same time).
+    template<bool LARGE, typename T>
     __device__ __forceinline__ void store_part(T* p, uint32_t left, s16x8 c) {
-        if (left >= (uint32_t) kUnit<T>) *reinterpret_cast<typename UnitOf<T>::mem*>(p) = __builtin_bit_cast(typename UnitOf<T>::mem, c);
-        else {
+        if (left >= (uint32_t) kUnit<T>) {
+            auto* to = reinterpret_cast<typename UnitOf<T>::mem*>(p);
+            if (LARGE) __builtin_nontemporal_store(__builtin_bit_cast(typename UnitOf<T>::mem, c), to);
+            else
+                *to = __builtin_bit_cast(typename UnitOf<T>::mem, c);
+        } else {
             T v[kUnit<T>];
             *reinterpret_cast<s16x8*>(v) = c;
 #pragma unroll
@@ -311,27 +324,40 @@ namespace splahip {
         RowTiles       tiles{};
         const uint32_t m_tiles = (g.m + BM - 1) / BM;// kMatrixGrad: row tiles of an expert
         if (FORM != kMatrixGrad) tiles = row_tiles_of(BM, g.n_experts, g.n_places, g.offsets);
-        const Patches  patches = patches_of(FORM == kMatrixGrad ? g.n_experts * m_tiles : tiles.total, col_tiles);
-        const uint32_t team = gridDim.x / 8;// (the grid is a multiple of 8)
+        // The tiles go out in runs of RUN neighbours, a run to RUN workgroups of one XCD (workgroup b runs in XCD b % 8), whose L2 then holds what they share; the runs go to
+        // such groups in turn.  kForward, kRowGrad: every tile costs the same and a run fills an XCD.  kMatrixGrad: a tile's cost is its expert's number of rows;
+        // the experts go out by falling number, there and back over the groups, in shorter runs (one expert's tiles on one XCD made it the last by a third).
+        constexpr uint32_t RUN = FORM == kMatrixGrad ? 8 : 32, HIGH = FORM == kMatrixGrad ? 2 : 4;
+        const uint32_t     groups = gridDim.x / RUN, group = blockIdx.x / 8 / RUN * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % RUN;// (the grid is a multiple of 8 RUN)
+        const uint32_t     n_tiles = (FORM == kMatrixGrad ? g.n_experts * m_tiles : tiles.total) * col_tiles;
+        const bool         ranked = FORM == kMatrixGrad && g.n_experts <= 64;
+        uint32_t           rank = 0;
+        if (ranked && lane < g.n_experts) {
+            const uint32_t begin = bounded(g.offsets, lane, g.n_experts, g.n_places), end = bounded(g.offsets, lane + 1, g.n_experts, g.n_places);
+            rank                 = end > begin ? end - begin : 0u;
+        }
+        if (ranked) rank = rank_by_rows(rank, g.n_experts);
 
         // the tile at hand
         const T *      A, *B;
         T*             C;
         uint32_t       rows, cols, depth, steps, whole;
         uint32_t       off_a[LOADS], off_b[LOADS];
-        // the XCD's tiles are numbered patch by patch
-        const uint32_t area = patches.width * patches.height;
-        uint32_t       at   = blockIdx.x / 8;
-        auto           next = [&]() -> bool {
-            for (;; at += team) {
-                const uint32_t p = at / area * 8 + blockIdx.x % 8, in = at % area;
-                if (p >= patches.count) return false;
-                const uint32_t row = p / patches.wide * patches.height + in / patches.width, col = p % patches.wide * patches.width + in % patches.width;
-                if (row >= patches.row_tiles || col >= patches.col_tiles) continue;
-                const uint32_t n0 = col * BN;
+        uint32_t round = 0;
+        auto     next = [&]() -> bool {
+            for (;;) {
+                const uint64_t run = (uint64_t) round * groups + (FORM == kMatrixGrad && (round & 1u) ? groups - 1 - group : group);
+                if ((uint64_t) round * groups * RUN >= n_tiles) return false;
+                ++round;
+                if (run * RUN + in >= n_tiles) continue;
+                const uint32_t t = (uint32_t) run * RUN + in;
+                const TileAt   at = FORM == kMatrixGrad ? tile_at<HIGH>(t % (m_tiles * col_tiles), m_tiles, col_tiles) : tile_at<HIGH>(t, tiles.total, col_tiles);
+                const uint32_t n0 = at.col * BN;
                 cols              = min(BN, g.n - n0);
                 if (FORM == kMatrixGrad) {
-                    const uint32_t expert = row / m_tiles, m0 = row % m_tiles * BM;
+                    uint32_t expert = t / (m_tiles * col_tiles);
+                    if (ranked) expert = __ffsll((unsigned long long) __ballot(lane < g.n_experts && rank == expert)) - 1;
+                    const uint32_t m0 = at.row * BM;
                     const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
                     rows                 = min(BM, g.m - m0);
                     depth                = end > begin ? end - begin : 0u;
@@ -339,7 +365,7 @@ namespace splahip {
                     B = static_cast<const T*>(g.b) + (size_t) begin * g.n + n0;
                     C = static_cast<T*>(g.c) + ((size_t) expert * g.m + m0) * g.n + n0;
                 } else {
-                    const RowTile  t = row_tile(tiles, row, BM, g.n_experts, g.n_places, g.offsets);
+                    const RowTile  t = row_tile(tiles, at.row, BM, g.n_experts, g.n_places, g.offsets);
                     const uint32_t e = min(t.expert, g.n_experts - 1);
                     rows             = t.rows;
                     depth            = t.expert < g.n_experts ? g.k : 0u;
@@ -354,7 +380,6 @@ namespace splahip {
                 asm volatile("" : "+s"(sa), "+s"(sb));
                 SlabA::offsets(sa, rows, off_a);
                 SlabB::offsets(sb, cols, off_b);
-                at += team;
                 return true;
             }
         };
@@ -502,7 +527,7 @@ namespace splahip {
                             s16x8          c;
                             __builtin_memcpy(&c, __builtin_assume_aligned(turn + row * kTurnCols + (unit ^ swz(row)) * kUnit<T>, 16), 16);
                             const uint32_t gm = wm + i * 32 + row, gn = wn + j0 * 32 + unit * kUnit<T>;
-                            if (gm < out_rows && gn < out_cols) store_part(out + (size_t) gm * ldc + gn, out_cols - gn, c);
+                            if (gm < out_rows && gn < out_cols) store_part<(BM > 128)>(out + (size_t) gm * ldc + gn, out_cols - gn, c);
                         }
                         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                         __builtin_amdgcn_wave_barrier();
@@ -516,7 +541,7 @@ namespace splahip {
 #pragma unroll
                         for (uint32_t v = 0; v < 16; v += 4) {
                             const uint32_t gm = wm + i * 32 + (lane & 31u), gn = wn + j * 32 + v * 2 + (lane >> 5) * 4;
-                            if (gm < out_rows && gn < out_cols) store_part(out + (size_t) gm * ldc + gn, out_cols - gn, __builtin_bit_cast(s16x8, quad(i, j, v)));
+                            if (gm < out_rows && gn < out_cols) store_part<(BM > 128)>(out + (size_t) gm * ldc + gn, out_cols - gn, __builtin_bit_cast(s16x8, quad(i, j, v)));
                         }
             }
         }
