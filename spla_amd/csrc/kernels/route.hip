@@ -16,10 +16,11 @@ namespace splahip {
     constexpr uint32_t kMaxExperts = 2048;
 
     // ---- the sort: a stable counting sort ------------------------------------------------------------------------------------------------------------
-    // A workgroup owns kSortTile consecutive entries, each of its four wavefronts a quarter of them.  Entry i's position is
+    // A workgroup owns kSortTile consecutive entries, each of its eight wavefronts an eighth of them.  Entry i's position is
     //   offsets[e] + (entries of e in earlier tiles) + (in earlier wavefronts of the tile) + (in earlier steps of the wavefront) + (in lower lanes of the step),
-    // the last by a ballot per bit of the expert's number.
-    constexpr uint32_t kSortThreads = 256, kSortWaves = kSortThreads / 64, kSortTile = 2048, kSortSteps = kSortTile / kSortThreads;
+    // the last by a ballot per bit of the expert's number.  Three launches (count, scan over the tiles, place); a tile's entries are brought into order in LDS first, so
+    // that `order` is written in runs.  Floor: 12 bytes per entry; what is left is the launches and the latency of each.
+    constexpr uint32_t kSortThreads = 512, kSortWaves = kSortThreads / 64, kSortTile = 4096, kSortSteps = kSortTile / kSortThreads;
 
     __device__ __forceinline__ uint64_t lanes_alike(uint32_t key, bool valid, uint32_t bits) {
         uint64_t m = __ballot(valid);
@@ -30,11 +31,12 @@ namespace splahip {
         return m;
     }
 
-    __global__ __launch_bounds__(256) void route_count_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t n_tiles, const int32_t* __restrict__ experts,
-                                                              uint32_t* __restrict__ counts) {
-        extern __shared__ uint32_t hist[];
+    // counts[tile, e]
+    __global__ __launch_bounds__(512) void route_count_kernel(uint32_t n_entries, uint32_t n_experts, const int32_t* __restrict__ experts, uint32_t* __restrict__ counts) {
+        __shared__ uint32_t hist[kMaxExperts];
         for (uint32_t e = threadIdx.x; e < n_experts; e += kSortThreads) hist[e] = 0;
         __syncthreads();
+#pragma unroll
         for (uint32_t s = 0; s < kSortSteps; ++s) {
             const uint32_t i = blockIdx.x * kSortTile + s * kSortThreads + threadIdx.x;
             if (i < n_entries) {
@@ -43,7 +45,7 @@ namespace splahip {
             }
         }
         __syncthreads();
-        for (uint32_t e = threadIdx.x; e < n_experts; e += kSortThreads) counts[(size_t) e * n_tiles + blockIdx.x] = hist[e];
+        for (uint32_t e = threadIdx.x; e < n_experts; e += kSortThreads) counts[(size_t) blockIdx.x * n_experts + e] = hist[e];
     }
 
     // exclusive scan of one value per thread over the workgroup; total returned through `sum`
@@ -70,19 +72,101 @@ namespace splahip {
         return before + inc - x;
     }
 
-    // one workgroup per expert: its tiles' counts become exclusive prefixes, their sum the expert's total
-    __global__ __launch_bounds__(256) void route_scan_kernel(uint32_t n_tiles, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
-        uint32_t* mine = counts + (size_t) blockIdx.x * n_tiles;
-        uint32_t  base = 0;
-        for (uint32_t t0 = 0; t0 < n_tiles; t0 += 256) {
-            const uint32_t t = t0 + threadIdx.x;
-            const uint32_t c = t < n_tiles ? mine[t] : 0u;
-            uint32_t       all;
-            const uint32_t ex = block_exclusive<256>(c, &all);
-            if (t < n_tiles) mine[t] = base + ex;
-            base += all;
+    // 64 experts a workgroup, one per lane; the wavefronts share the tiles in contiguous parts: the counts become exclusive prefixes over the tiles, their sums the totals
+    __global__ __launch_bounds__(1024) void route_scan_kernel(uint32_t n_tiles, uint32_t n_experts, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
+        __shared__ uint32_t part[16][64];
+        const uint32_t      lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+        const uint32_t      per = (n_tiles + 15) / 16, t0 = min(wave * per, n_tiles), t1 = min(t0 + per, n_tiles);
+        uint32_t            sum = 0;
+        if (e < n_experts)
+#pragma unroll 8
+            for (uint32_t t = t0; t < t1; ++t) sum += counts[(size_t) t * n_experts + e];
+        part[wave][lane] = sum;
+        __syncthreads();
+        uint32_t at = 0, all = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < 16; ++w) {
+            at += w < wave ? part[w][lane] : 0u;
+            all += part[w][lane];
         }
-        if (threadIdx.x == 0) totals[blockIdx.x] = base;
+        if (e >= n_experts) return;
+        if (wave == 0) totals[e] = all;
+#pragma unroll 8
+        for (uint32_t t = t0; t < t1; ++t) {
+            const uint32_t c                       = counts[(size_t) t * n_experts + e];
+            counts[(size_t) t * n_experts + e] = at;
+            at += c;
+        }
+    }
+
+    // EXPERTS >= n_experts: the size of the tables in LDS
+    template<uint32_t EXPERTS>
+    __global__ __launch_bounds__(512) void route_place_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t bits, const int32_t* __restrict__ experts,
+                                                              const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals, uint32_t* __restrict__ offsets,
+                                                              int32_t* __restrict__ order, int32_t* __restrict__ place) {
+        __shared__ uint32_t wave_count[kSortWaves][EXPERTS];
+        __shared__ uint32_t shift[EXPERTS];// place of an entry of e - its place in the tile's order
+        __shared__ uint32_t entry[kSortTile], place_of[kSortTile];
+        const uint32_t      lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, first = blockIdx.x * kSortTile + wave * kSortSteps * 64;
+        uint32_t            mine[kSortSteps];
+#pragma unroll
+        for (uint32_t s = 0; s < kSortSteps; ++s) {
+            const uint32_t i = first + s * 64 + lane;
+            mine[s]          = i < n_entries ? (uint32_t) experts[i] : ~0u;
+        }
+        for (uint32_t e = lane; e < n_experts; e += 64) wave_count[wave][e] = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t s = 0; s < kSortSteps; ++s)
+            if (mine[s] < n_experts) atomicAdd(&wave_count[wave][mine[s]], 1u);
+        __syncthreads();
+        uint32_t run = 0, here = 0;
+        for (uint32_t e0 = 0; e0 < n_experts; e0 += kSortThreads) {
+            const uint32_t e = e0 + threadIdx.x;
+            uint32_t       all, in_tile = 0, count = 0;
+            const uint32_t at = run + block_exclusive<kSortThreads>(e < n_experts ? totals[e] : 0u, &all);
+            run += all;
+            if (e < n_experts)
+#pragma unroll
+                for (uint32_t w = 0; w < kSortWaves; ++w) count += wave_count[w][e];
+            in_tile = here + block_exclusive<kSortThreads>(count, &all);
+            here += all;
+            if (e < n_experts) {
+                if (blockIdx.x == 0) offsets[e] = at;
+                shift[e] = at + (n_entries ? counts[(size_t) blockIdx.x * n_experts + e] : 0u) - in_tile;
+                for (uint32_t w = 0; w < kSortWaves; ++w) {
+                    const uint32_t c = wave_count[w][e];
+                    wave_count[w][e] = in_tile;
+                    in_tile += c;
+                }
+            }
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) offsets[n_experts] = run;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t s = 0; s < kSortSteps; ++s) {// (a wavefront's own counts only: its LDS accesses stay in program order)
+            const uint32_t i = first + s * 64 + lane, e = mine[s];
+            const bool     valid = e < n_experts;
+            const uint64_t alike = lanes_alike(e, valid, bits);
+            const uint32_t below = __popcll(alike & ((1ull << lane) - 1ull));
+            uint32_t       p     = ~0u;
+            if (valid) {
+                const uint32_t at = *(volatile uint32_t*) &wave_count[wave][e] + below;
+                p                 = at + shift[e];
+                entry[at]         = i;
+                place_of[at]      = p;
+                if (below == 0) *(volatile uint32_t*) &wave_count[wave][e] = at + (uint32_t) __popcll(alike);
+            }
+            if (i < n_entries) place[i] = (int32_t) p;
+        }
+        __syncthreads();
+        for (uint32_t at = threadIdx.x; at < here; at += kSortThreads) order[place_of[at]] = (int32_t) entry[at];
+        // order behind the last entry: this tile's share of those places
+#pragma unroll
+        for (uint32_t s = 0; s < kSortSteps; ++s) {
+            const uint32_t i = first + s * 64 + lane;
+            if (i < n_entries && i >= run) order[i] = -1;
+        }
     }
 
     // a wavefront's entries, 64 at a time from `first`: mine[e] (LDS) = where its next entry of e goes
@@ -103,60 +187,6 @@ namespace splahip {
                 if (below == 0) *(volatile uint32_t*) &mine[e] = p + (uint32_t) __popcll(alike);
             }
         }
-    }
-
-    // positions of the tile's entries; base[e] (LDS) = where the tile's first entry of e goes.  `waves` x n_experts words of LDS behind it.
-    __device__ __forceinline__ void place_tile(uint32_t tile, uint32_t n_entries, uint32_t n_experts, uint32_t bits, const int32_t* __restrict__ experts,
-                                               int32_t* __restrict__ order, int32_t* __restrict__ place, const uint32_t* base, uint32_t* wave_count, uint32_t n_waves,
-                                               uint32_t steps) {
-        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-        uint32_t*      mine  = wave_count + wave * n_experts;
-        const uint32_t first = tile * n_waves * steps * 64 + wave * steps * 64;
-        for (uint32_t e = lane; e < n_experts; e += 64) mine[e] = 0;
-        __syncthreads();
-        for (uint32_t s = 0; s < steps; ++s) {
-            const uint32_t i = first + s * 64 + lane;
-            const uint32_t e = i < n_entries ? (uint32_t) experts[i] : ~0u;
-            if (e < n_experts) atomicAdd(&mine[e], 1u);
-        }
-        __syncthreads();
-        // the wavefronts' counts -> where each wavefront's first entry of e goes
-        for (uint32_t e = threadIdx.x; e < n_experts; e += blockDim.x) {
-            uint32_t at = base[e];
-            for (uint32_t w = 0; w < n_waves; ++w) {
-                const uint32_t c               = wave_count[w * n_experts + e];
-                wave_count[w * n_experts + e] = at;
-                at += c;
-            }
-        }
-        __syncthreads();
-        place_wave(first, steps, n_entries, n_experts, bits, experts, order, place, mine);
-    }
-
-    __global__ __launch_bounds__(256) void route_place_kernel(uint32_t n_entries, uint32_t n_experts, uint32_t n_tiles, uint32_t bits, const int32_t* __restrict__ experts,
-                                                              const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals, uint32_t* __restrict__ offsets,
-                                                              int32_t* __restrict__ order, int32_t* __restrict__ place) {
-        extern __shared__ uint32_t lds[];
-        uint32_t*                  base = lds;// n_experts
-        uint32_t                   run  = 0;
-        for (uint32_t e0 = 0; e0 < n_experts; e0 += kSortThreads) {
-            const uint32_t e = e0 + threadIdx.x;
-            uint32_t       all;
-            const uint32_t at = run + block_exclusive<kSortThreads>(e < n_experts ? totals[e] : 0u, &all);
-            if (e < n_experts) {
-                base[e] = at + counts[(size_t) e * n_tiles + blockIdx.x];
-                if (blockIdx.x == 0) offsets[e] = at;
-            }
-            run += all;
-        }
-        if (blockIdx.x == 0 && threadIdx.x == 0) offsets[n_experts] = run;
-        // order behind the last entry: this tile's share of those places
-        for (uint32_t s = 0; s < kSortSteps; ++s) {
-            const uint32_t i = blockIdx.x * kSortTile + s * kSortThreads + threadIdx.x;
-            if (i < n_entries && i >= run) order[i] = -1;
-        }
-        __syncthreads();
-        place_tile(blockIdx.x, n_entries, n_experts, bits, experts, order, place, base, lds + n_experts, kSortWaves, kSortSteps);
     }
 
     // The whole sort in one workgroup of 16 wavefronts: a wavefront counts and places a contiguous part of the entries.
@@ -357,9 +387,10 @@ extern "C" int splahip_route_sort(uint32_t n_rows, uint32_t per_row, uint32_t n_
     }
     uint32_t* counts = static_cast<uint32_t*>(d_workspace);
     uint32_t* totals = counts + (size_t) n_experts * tiles;
-    if (tiles) route_count_kernel<<<tiles, kSortThreads, n_experts * 4, s>>>(n, n_experts, tiles, d_experts, counts);
-    route_scan_kernel<<<n_experts, 256, 0, s>>>(tiles, counts, totals);
-    route_place_kernel<<<tiles ? tiles : 1, kSortThreads, n_experts * 4 * (1 + kSortWaves), s>>>(n, n_experts, tiles, bits, d_experts, counts, totals, d_offsets, d_order, d_place);
+    if (tiles) route_count_kernel<<<tiles, kSortThreads, 0, s>>>(n, n_experts, d_experts, counts);
+    route_scan_kernel<<<(n_experts + 63) / 64, 1024, 0, s>>>(tiles, n_experts, counts, totals);
+    auto* place_kernel = n_experts <= 512 ? route_place_kernel<512> : route_place_kernel<kMaxExperts>;
+    place_kernel<<<tiles ? tiles : 1, kSortThreads, 0, s>>>(n, n_experts, bits, d_experts, counts, totals, d_offsets, d_order, d_place);
     SPLAHIP_TRY(hipGetLastError());
     return SPLAHIP_OK;
 }

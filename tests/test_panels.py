@@ -109,6 +109,6 @@ def test_clip_refuses_overlaps_and_limits():
 
 def test_workspaces_cover_the_largest():
     assert _lib.call("splahip_route_sort_workspace", 1 << 16, 2, 8) >= 32
-    assert _lib.call("splahip_route_sort_workspace", (1 << 31) // 8 - 1, 8, 128) >= ((1 << 31) - 8) // 2048 * 128 * 4
+    assert _lib.call("splahip_route_sort_workspace", (1 << 31) // 8 - 1, 8, 128) >= ((1 << 31) - 8) // 4096 * 128 * 4
     assert _lib.call("splahip_global_norm_workspace", 0, (C.c_uint64 * 1)()) >= 8
     assert _lib.call("splahip_global_norm_workspace", 2, (C.c_uint64 * 2)(0, 1)) >= 16
