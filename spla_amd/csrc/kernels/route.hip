@@ -11,6 +11,8 @@
 // Every sum has a fixed order: results are the same from run to run.
 #include "panel.hpp"
 
+#include <type_traits>
+
 namespace splahip {
 
     constexpr uint32_t kMaxExperts = 2048;
@@ -237,105 +239,158 @@ namespace splahip {
         return r;
     }
 
-    // x is read once and written to each of the row's places (4 rows of the panel would otherwise be fetched from as many distant places of the order).
-    template<typename T, bool WEIGHTED>
+    // one unit of a row whose end may cut it; LARGE panels are streamed past the caches
+    template<typename T, bool LARGE>
+    __device__ __forceinline__ typename UnitOf<T>::mem unit_at(const T* __restrict__ p, uint32_t left) {
+        typename UnitOf<T>::mem v;
+        if (left >= (uint32_t) kUnit<T>) {
+            auto* from = reinterpret_cast<const typename UnitOf<T>::mem*>(p);
+            v          = LARGE ? __builtin_nontemporal_load(from) : *from;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kUnit<T>; ++i) v[i] = (uint32_t) i < left ? p[i] : (T) 0.0f;
+        }
+        return v;
+    }
+    template<typename T, bool LARGE>
+    __device__ __forceinline__ void put_unit(T* __restrict__ p, uint32_t left, typename UnitOf<T>::mem v) {
+        if (left >= (uint32_t) kUnit<T>) {
+            auto* to = reinterpret_cast<typename UnitOf<T>::mem*>(p);
+            if (LARGE) __builtin_nontemporal_store(v, to);
+            else
+                *to = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kUnit<T>; ++i)
+                if ((uint32_t) i < left) p[i] = v[i];
+        }
+    }
+    template<typename T>
+    __device__ __forceinline__ typename UnitOf<T>::mem scaled(typename UnitOf<T>::mem v, float w) {
+#pragma unroll
+        for (int i = 0; i < kUnit<T>; ++i) v[i] = (T) (w * (float) v[i]);
+        return v;
+    }
+    // rows [first, n_places) of a panel become 0; `rows` rows at a time, `lanes` threads each, `workers` workgroups
+    template<typename T>
+    __device__ __forceinline__ void clear_rows(T* __restrict__ out, uint32_t first, uint32_t n_places, uint32_t width, uint32_t worker, uint32_t workers, uint32_t shift) {
+        constexpr uint32_t U = kUnit<T>;
+        const uint32_t     lanes = 1u << shift, sub = threadIdx.x & (lanes - 1u), rows = 256u >> shift;
+        for (uint64_t p = (uint64_t) first + worker * rows + (threadIdx.x >> shift); p < n_places; p += (uint64_t) workers * rows)
+            for (uint32_t c = sub * U; c < width; c += lanes * U) put_unit<T, false>(out + p * width + c, width - c, typename UnitOf<T>::mem{});
+    }
+
+    // x is read once and written to each of the row's places (gathered instead, a row would be fetched once per entry from places far apart in time).
+    template<typename T, bool WEIGHTED, bool LARGE>
     __global__ __launch_bounds__(256) void route_rows_kernel(uint32_t n_rows, uint32_t per_row, uint32_t width, uint32_t n_experts, uint32_t row_blocks, uint32_t shift,
                                                              const uint32_t* __restrict__ offsets, const int32_t* __restrict__ place, const float* __restrict__ weights,
                                                              const T* __restrict__ x, T* __restrict__ out) {
         constexpr uint32_t U        = kUnit<T>;
         const uint32_t     lanes    = 1u << shift, sub = threadIdx.x & (lanes - 1u);
         const uint32_t     n_places = n_rows * per_row;
-        const uint32_t     rows     = 256u >> shift;
-        if (blockIdx.x >= row_blocks) {// the rows behind the last entry
-            const uint32_t end = min(offsets[n_experts], n_places);
-            for (uint64_t p = (uint64_t) end + (blockIdx.x - row_blocks) * rows + (threadIdx.x >> shift); p < n_places; p += (uint64_t) (gridDim.x - row_blocks) * rows)
-                for (uint32_t c = sub * U; c < width; c += lanes * U) {
-                    const float zero[U] = {};
-                    store_unit<T>(out + p * width + c, width - c, zero);
-                }
+        if (blockIdx.x >= row_blocks) {
+            clear_rows(out, min(offsets[n_experts], n_places), n_places, width, blockIdx.x - row_blocks, gridDim.x - row_blocks, shift);
             return;
         }
-        const uint32_t r = blockIdx.x * rows + (threadIdx.x >> shift);
+        const uint32_t r = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
         if (r >= n_rows) return;
         for (uint32_t c = sub * U; c < width; c += lanes * U) {
-            float v[U];
-            load_unit<T>(x + (size_t) r * width + c, width - c, v);
+            const auto v = unit_at<T, LARGE>(x + (size_t) r * width + c, width - c);
             for (uint32_t j = 0; j < per_row; ++j) {
                 const uint32_t i = r * per_row + j;
                 const uint32_t p = (uint32_t) place[i];
                 if (p >= n_places) continue;
-                if (WEIGHTED) {
-                    const float w = weights[i];
-                    float       s[U];
-#pragma unroll
-                    for (uint32_t q = 0; q < U; ++q) s[q] = w * v[q];
-                    store_unit<T>(out + (size_t) p * width + c, width - c, s);
-                } else {
-                    store_unit<T>(out + (size_t) p * width + c, width - c, v);
-                }
+                put_unit<T, LARGE>(out + (size_t) p * width + c, width - c, WEIGHTED ? scaled<T>(v, weights[i]) : v);
             }
         }
     }
 
-    template<typename T, bool WEIGHTED>
+    // four entries' units under way
+    template<typename T, bool WEIGHTED, bool LARGE>
     __global__ __launch_bounds__(256) void route_back_kernel(uint32_t n_rows, uint32_t per_row, uint32_t width, uint32_t shift, const int32_t* __restrict__ place,
                                                              const float* __restrict__ weights, const T* __restrict__ y, T* __restrict__ out) {
-        constexpr uint32_t U        = kUnit<T>;
+        constexpr uint32_t U        = kUnit<T>, AHEAD = 4;
         const uint32_t     lanes    = 1u << shift, sub = threadIdx.x & (lanes - 1u);
         const uint32_t     n_places = n_rows * per_row;
         const uint32_t     r        = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
         if (r >= n_rows) return;
         for (uint32_t c = sub * U; c < width; c += lanes * U) {
             float s[U] = {};
-            for (uint32_t j = 0; j < per_row; ++j) {
-                const uint32_t i = r * per_row + j;
-                const uint32_t p = (uint32_t) place[i];
-                if (p >= n_places) continue;// (no entry: its weight does not count either)
-                float v[U];
-                load_unit<T>(y + (size_t) p * width + c, width - c, v);
-                const float w = WEIGHTED ? weights[i] : 1.0f;
+            for (uint32_t j0 = 0; j0 < per_row; j0 += AHEAD) {
+                typename UnitOf<T>::mem v[AHEAD];
+                bool                    here[AHEAD];// (no entry: its weight does not count either)
 #pragma unroll
-                for (uint32_t q = 0; q < U; ++q) s[q] = WEIGHTED ? fmaf(w, v[q], s[q]) : s[q] + v[q];
+                for (uint32_t j = 0; j < AHEAD; ++j) {
+                    const uint32_t p = j0 + j < per_row ? (uint32_t) place[r * per_row + j0 + j] : ~0u;
+                    here[j]          = p < n_places;
+                    if (here[j]) v[j] = unit_at<T, LARGE>(y + (size_t) p * width + c, width - c);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < AHEAD; ++j)
+                    if (here[j]) {
+                        const float w = WEIGHTED ? weights[r * per_row + j0 + j] : 1.0f;
+#pragma unroll
+                        for (uint32_t q = 0; q < U; ++q) s[q] = WEIGHTED ? fmaf(w, (float) v[j][q], s[q]) : s[q] + (float) v[j][q];
+                    }
             }
-            store_unit<T>(out + (size_t) r * width + c, width - c, s);
+            typename UnitOf<T>::mem o;
+#pragma unroll
+            for (uint32_t q = 0; q < U; ++q) o[q] = (T) s[q];
+            put_unit<T, false>(out + (size_t) r * width + c, width - c, o);
         }
     }
 
-    // one wavefront per row: the products of the entry's weight are reduced inside it
-    template<typename T>
+    // One wavefront per row: an entry's weight gradient is reduced inside it.  UNITS units of dout's row stay in its registers (0: a row longer than eight per lane is read
+    // again for every entry).
+    template<typename T, uint32_t UNITS, bool LARGE>
     __global__ __launch_bounds__(256) void route_back_grad_kernel(uint32_t n_rows, uint32_t per_row, uint32_t width, uint32_t n_experts, uint32_t row_blocks,
                                                                   const uint32_t* __restrict__ offsets, const int32_t* __restrict__ place,
                                                                   const float* __restrict__ weights, const T* __restrict__ y, const T* __restrict__ dout,
                                                                   T* __restrict__ dy, float* __restrict__ dweights) {
-        constexpr uint32_t U        = kUnit<T>;
+        constexpr uint32_t U        = kUnit<T>, KEPT = UNITS ? UNITS : 1;
         const uint32_t     lane     = threadIdx.x & 63u, wave = threadIdx.x >> 6;
         const uint32_t     n_places = n_rows * per_row;
         if (blockIdx.x >= row_blocks) {
-            const uint32_t end = min(offsets[n_experts], n_places);
-            for (uint64_t p = (uint64_t) end + (blockIdx.x - row_blocks) * 4 + wave; p < n_places; p += (uint64_t) (gridDim.x - row_blocks) * 4)
-                for (uint32_t c = lane * U; c < width; c += 64 * U) {
-                    const float zero[U] = {};
-                    store_unit<T>(dy + p * width + c, width - c, zero);
-                }
+            clear_rows(dy, min(offsets[n_experts], n_places), n_places, width, blockIdx.x - row_blocks, gridDim.x - row_blocks, 6);
             return;
         }
         const uint32_t r = blockIdx.x * 4 + wave;
         if (r >= n_rows) return;
+        const T*                grow = dout + (size_t) r * width;
+        typename UnitOf<T>::mem kept[KEPT];
+        if (UNITS)
+#pragma unroll
+            for (uint32_t u = 0; u < KEPT; ++u) {
+                const uint32_t c = (u * 64 + lane) * U;
+                if (c < width) kept[u] = unit_at<T, LARGE>(grow + c, width - c);
+            }
         for (uint32_t j = 0; j < per_row; ++j) {
             const uint32_t i   = r * per_row + j;
             const uint32_t p   = (uint32_t) place[i];
             float          dot = 0.0f;
             if (p < n_places) {
-                const float w = weights[i];
-                for (uint32_t c = lane * U; c < width; c += 64 * U) {
-                    float g[U], v[U];
-                    load_unit<T>(dout + (size_t) r * width + c, width - c, g);
-                    load_unit<T>(y + (size_t) p * width + c, width - c, v);
+                const float w    = weights[i];
+                const T*    yrow = y + (size_t) p * width;
+                T*          drow = dy + (size_t) p * width;
+                auto        part = [&](uint32_t c, typename UnitOf<T>::mem g, typename UnitOf<T>::mem v) {
 #pragma unroll
-                    for (uint32_t q = 0; q < U; ++q) dot = fmaf(g[q], v[q], dot);
+                    for (uint32_t q = 0; q < U; ++q) dot = fmaf((float) g[q], (float) v[q], dot);
+                    put_unit<T, LARGE>(drow + c, width - c, scaled<T>(g, w));
+                };
+                if (UNITS) {
+                    typename UnitOf<T>::mem v[KEPT];
 #pragma unroll
-                    for (uint32_t q = 0; q < U; ++q) g[q] *= w;
-                    store_unit<T>(dy + (size_t) p * width + c, width - c, g);
+                    for (uint32_t u = 0; u < KEPT; ++u) {
+                        const uint32_t c = (u * 64 + lane) * U;
+                        if (c < width) v[u] = unit_at<T, LARGE>(yrow + c, width - c);
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < KEPT; ++u) {
+                        const uint32_t c = (u * 64 + lane) * U;
+                        if (c < width) part(c, kept[u], v[u]);
+                    }
+                } else {
+                    for (uint32_t c = lane * U; c < width; c += 64 * U) part(c, unit_at<T, false>(grow + c, width - c), unit_at<T, LARGE>(yrow + c, width - c));
                 }
 #pragma unroll
                 for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
@@ -355,6 +410,8 @@ namespace splahip {
         return SPLAHIP_OK;
     }
     constexpr uint32_t kTailBlocks = 128;// workgroups that clear the rows behind the last entry (none of them: they return at once)
+    // A panel that the caches (256 MB behind the L2s) do not hold along with what else is read: streamed past the L2 (the gradient of 65536 x 2048 bf16 rows 125 -> 119 us).
+    static bool large_panel(uint32_t n_places, uint32_t width, size_t element) { return (uint64_t) n_places * width * element > (128ull << 20); }
 
 }// namespace splahip
 
@@ -410,9 +467,9 @@ extern "C" int splahip_route_rows(int panel_type, uint32_t n_rows, uint32_t per_
         const uint32_t rows  = 256u >> sh.shift, blocks = (n_rows + rows - 1) / rows;
         auto*          x     = static_cast<const T*>(d_x);
         auto*          out   = static_cast<T*>(d_out);
-        if (d_weights) route_rows_kernel<T, true><<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, sh.shift, d_offsets, d_place, d_weights, x, out);
-        else
-            route_rows_kernel<T, false><<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, sh.shift, d_offsets, d_place, d_weights, x, out);
+        const bool     large = large_panel(n_rows * per_row, width, sizeof(T));
+        auto*          kernel = d_weights ? (large ? route_rows_kernel<T, true, true> : route_rows_kernel<T, true, false>) : (large ? route_rows_kernel<T, false, true> : route_rows_kernel<T, false, false>);
+        kernel<<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, sh.shift, d_offsets, d_place, d_weights, x, out);
     });
     SPLAHIP_TRY(hipGetLastError());
     return SPLAHIP_OK;
@@ -433,9 +490,9 @@ extern "C" int splahip_route_back(int panel_type, uint32_t n_rows, uint32_t per_
         const uint32_t rows = 256u >> sh.shift, blocks = (n_rows + rows - 1) / rows;
         auto*          y    = static_cast<const T*>(d_y);
         auto*          out  = static_cast<T*>(d_out);
-        if (d_weights) route_back_kernel<T, true><<<blocks, 256, 0, s>>>(n_rows, per_row, width, sh.shift, d_place, d_weights, y, out);
-        else
-            route_back_kernel<T, false><<<blocks, 256, 0, s>>>(n_rows, per_row, width, sh.shift, d_place, d_weights, y, out);
+        const bool     large = large_panel(n_rows * per_row, width, sizeof(T));
+        auto*          kernel = d_weights ? (large ? route_back_kernel<T, true, true> : route_back_kernel<T, true, false>) : (large ? route_back_kernel<T, false, true> : route_back_kernel<T, false, false>);
+        kernel<<<blocks, 256, 0, s>>>(n_rows, per_row, width, sh.shift, d_place, d_weights, y, out);
     });
     SPLAHIP_TRY(hipGetLastError());
     return SPLAHIP_OK;
@@ -453,8 +510,16 @@ extern "C" int splahip_route_back_grad(int panel_type, uint32_t n_rows, uint32_t
     const uint32_t blocks = (n_rows + 3) / 4;
     panel_dispatch(panel_type, [&](auto zero) {
         using T = decltype(zero);
-        route_back_grad_kernel<T><<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, d_offsets, d_place, d_weights, static_cast<const T*>(d_y),
-                                                                       static_cast<const T*>(d_dout), static_cast<T*>(d_dy), d_dweights);
+        const uint32_t per_lane = (width + 64 * kUnit<T> - 1) / (64 * kUnit<T>);
+        const bool     large = large_panel(n_rows * per_row, width, sizeof(T));
+        auto           pick = [&](auto units) {
+            constexpr uint32_t N = decltype(units)::value;
+            return large ? route_back_grad_kernel<T, N, true> : route_back_grad_kernel<T, N, false>;
+        };
+        auto* kernel = per_lane <= 1 ? pick(std::integral_constant<uint32_t, 1>{}) : per_lane <= 2 ? pick(std::integral_constant<uint32_t, 2>{})
+                     : per_lane <= 4 ? pick(std::integral_constant<uint32_t, 4>{}) : per_lane <= 8 ? pick(std::integral_constant<uint32_t, 8>{}) : pick(std::integral_constant<uint32_t, 0>{});
+        kernel<<<blocks + kTailBlocks, 256, 0, s>>>(n_rows, per_row, width, n_experts, blocks, d_offsets, d_place, d_weights, static_cast<const T*>(d_y),
+                                                    static_cast<const T*>(d_dout), static_cast<T*>(d_dy), d_dweights);
     });
     SPLAHIP_TRY(hipGetLastError());
     return SPLAHIP_OK;
