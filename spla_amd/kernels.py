@@ -428,17 +428,18 @@ class _Words:
 
 
 def _arrays(name, tensors):
-    """address, length and type arrays of the tensors, all on one device"""
+    """address, length and type arrays of the tensors, all on one device, and the device"""
     try:
         types = _Words("i", [_PANEL_TYPE[t.dtype] for t in tensors])
-        same = len({t.device for t in tensors}) == 1 and tensors[0].is_cuda and all([t.is_contiguous() for t in tensors])
+        places = set(map(torch.Tensor.get_device, tensors))
+        fits = len(places) == 1 and places.pop() >= 0 and all(map(torch.Tensor.is_contiguous, tensors))
     except (AttributeError, KeyError, TypeError):
-        same = False
-    if not same:  # say which
+        fits = False
+    if not fits:  # say which
         for i, t in enumerate(tensors):
             _panel_type(f"{name}[{i}]", t)
             _checked(f"{name}[{i}]", t, t.dtype, t.shape, tensors[0].device)
-    return _Words("Q", [t.data_ptr() for t in tensors]), _Words("Q", [t.numel() for t in tensors]), types, tensors[0].device
+    return _Words("Q", list(map(torch.Tensor.data_ptr, tensors))), _Words("Q", list(map(torch.Tensor.numel, tensors))), types, tensors[0].device
 
 
 def global_norm(tensors) -> torch.Tensor:
@@ -456,7 +457,7 @@ def global_norm(tensors) -> torch.Tensor:
 
 
 def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None) -> torch.Tensor:
-    """Scale the tensors by min(1, limit / norm), in place or into the list `out` (same shapes and types), and return the norm before.  A norm that is not finite
+    """Scale the tensors by min(1, limit / norm), in place or into the list `out` (same lengths and types), and return the norm before.  A norm that is not finite
     scales nothing (the caller sees it in the result).  norm: a float32 scalar on the device to use instead (the norm over several devices' tensors, say)."""
     tensors = list(tensors)
     if not tensors:
@@ -467,10 +468,9 @@ def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None)
         out = list(out)
         if len(out) != len(tensors):
             raise ValueError(f"out: {len(tensors)} tensors expected, not {len(out)}")
-        out_ptrs, _, _, out_device = _arrays("out", out)
-        if out_device != device or [t.dtype for t in out] != [t.dtype for t in tensors] or [t.shape for t in out] != [t.shape for t in tensors]:
-            for i, (o, t) in enumerate(zip(out, tensors)):
-                _checked(f"out[{i}]", o, t.dtype, t.shape, device)
+        out_ptrs, out_lengths, out_types, out_device = _arrays("out", out)
+        if out_device != device or out_types.words != types.words or out_lengths.words != lengths.words:
+            raise ValueError("out: tensors of the same lengths, types and device as the tensors expected")
     if norm is not None:
         _checked("norm", norm, torch.float32, (), device)
         work, n_bytes, given = None, 0, 1
