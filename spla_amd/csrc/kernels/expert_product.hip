@@ -300,8 +300,16 @@ namespace splahip {
         }
     }
 
-    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC>
-    __global__ __launch_bounds__(WM* WN * 64, OCC) void product_kernel(const ProductArgs g, uint32_t col_tiles) {
+    template<typename T>
+    struct Tile {
+        const T *a, *b;
+        T*       c;
+        uint32_t rows, cols, depth;
+    };
+
+    // take(tile): the workgroup's next tile, false behind the last
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, typename TAKE>
+    __device__ __forceinline__ void run_tiles(const ProductArgs& g, T* lds, TAKE&& take) {
         constexpr uint32_t BN = BM, THREADS = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
         constexpr bool     A_DEPTH = FORM != kMatrixGrad, B_DEPTH = FORM == kForward;
         using SlabA                   = Slab<T, BM, THREADS, A_DEPTH, LOAD>;
@@ -313,75 +321,30 @@ namespace splahip {
         constexpr uint32_t kTurn = sizeof(T) == 2 ? TN : 1, kTurnCols = kTurn * 32, kRowUnits = kTurnCols / kUnit<T>;
         constexpr bool     kTurns = WM * WN * 32 * kTurnCols <= kSlab;
         constexpr uint32_t kStores = kTurns ? TM * (TN / kTurn) * 32 * kRowUnits / 64 : TM * TN * 4;
-        __shared__ __align__(1024) T slabs[kSlots][kSlab];
+        auto slabs = [&](uint32_t slot) { return lds + slot * kSlab; };
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const uint32_t wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
         const uint32_t stride_a = FORM == kMatrixGrad ? g.m : g.k, stride_b = FORM == kForward ? g.k : g.n;
         const size_t   move_a = A_DEPTH ? kStep<T> : (size_t) kStep<T> * stride_a, move_b = B_DEPTH ? kStep<T> : (size_t) kStep<T> * stride_b;
-        const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void*) slabs + wave * (64 * SlabA::kPiece);
+        const uint32_t lds0 = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) void*) lds + wave * (64 * SlabA::kPiece);
         constexpr uint32_t kSlabBytes = kSlab * sizeof(T);
 
-        RowTiles       tiles{};
-        const uint32_t m_tiles = (g.m + BM - 1) / BM;// kMatrixGrad: row tiles of an expert
-        if (FORM != kMatrixGrad) tiles = row_tiles_of(BM, g.n_experts, g.n_places, g.offsets);
-        // The tiles go out in runs of RUN neighbours, a run to RUN workgroups of one XCD (workgroup b runs in XCD b % 8), whose L2 then holds what they share; the runs go to
-        // such groups in turn.  kForward, kRowGrad: every tile costs the same and a run fills an XCD.  kMatrixGrad: a tile's cost is its expert's number of rows;
-        // the experts go out by falling number, there and back over the groups, in shorter runs (one expert's tiles on one XCD made it the last by a third).
-        constexpr uint32_t RUN = FORM == kMatrixGrad ? 8 : 32, HIGH = FORM == kMatrixGrad ? 2 : 4;
-        const uint32_t     groups = gridDim.x / RUN, group = blockIdx.x / 8 / RUN * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % RUN;// (the grid is a multiple of 8 RUN)
-        const uint32_t     n_tiles = (FORM == kMatrixGrad ? g.n_experts * m_tiles : tiles.total) * col_tiles;
-        const bool         ranked = FORM == kMatrixGrad && g.n_experts <= 64;
-        uint32_t           rank = 0;
-        if (ranked && lane < g.n_experts) {
-            const uint32_t begin = bounded(g.offsets, lane, g.n_experts, g.n_places), end = bounded(g.offsets, lane + 1, g.n_experts, g.n_places);
-            rank                 = end > begin ? end - begin : 0u;
-        }
-        if (ranked) rank = rank_by_rows(rank, g.n_experts);
-
         // the tile at hand
-        const T *      A, *B;
-        T*             C;
-        uint32_t       rows, cols, depth, steps, whole;
-        uint32_t       off_a[LOADS], off_b[LOADS];
-        uint32_t round = 0;
+        const T *A, *B;
+        T*       C;
+        uint32_t rows, cols, depth, steps, whole;
+        uint32_t off_a[LOADS], off_b[LOADS];
         auto     next = [&]() -> bool {
-            for (;;) {
-                const uint64_t run = (uint64_t) round * groups + (FORM == kMatrixGrad && (round & 1u) ? groups - 1 - group : group);
-                if ((uint64_t) round * groups * RUN >= n_tiles) return false;
-                ++round;
-                if (run * RUN + in >= n_tiles) continue;
-                const uint32_t t = (uint32_t) run * RUN + in;
-                const TileAt   at = FORM == kMatrixGrad ? tile_at<HIGH>(t % (m_tiles * col_tiles), m_tiles, col_tiles) : tile_at<HIGH>(t, tiles.total, col_tiles);
-                const uint32_t n0 = at.col * BN;
-                cols              = min(BN, g.n - n0);
-                if (FORM == kMatrixGrad) {
-                    uint32_t expert = t / (m_tiles * col_tiles);
-                    if (ranked) expert = __ffsll((unsigned long long) __ballot(lane < g.n_experts && rank == expert)) - 1;
-                    const uint32_t m0 = at.row * BM;
-                    const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
-                    rows                 = min(BM, g.m - m0);
-                    depth                = end > begin ? end - begin : 0u;
-                    A = static_cast<const T*>(g.a) + (size_t) begin * g.m + m0;
-                    B = static_cast<const T*>(g.b) + (size_t) begin * g.n + n0;
-                    C = static_cast<T*>(g.c) + ((size_t) expert * g.m + m0) * g.n + n0;
-                } else {
-                    const RowTile  t = row_tile(tiles, at.row, BM, g.n_experts, g.n_places, g.offsets);
-                    const uint32_t e = min(t.expert, g.n_experts - 1);
-                    rows             = t.rows;
-                    depth            = t.expert < g.n_experts ? g.k : 0u;
-                    A = static_cast<const T*>(g.a) + (size_t) t.row0 * g.k;
-                    B = static_cast<const T*>(g.b) + (FORM == kForward ? ((size_t) e * g.n + n0) * g.k : (size_t) e * g.n * g.k + n0);
-                    C = static_cast<T*>(g.c) + (size_t) t.row0 * g.n + n0;
-                }
-                A = uniform(A), B = uniform(B), C = uniform(C);
-                rows = __builtin_amdgcn_readfirstlane(rows), depth = __builtin_amdgcn_readfirstlane(depth);
-                steps = (depth + kStep<T> - 1) / kStep<T>, whole = depth / kStep<T>;
-                uint32_t sa = stride_a, sb = stride_b;// (opaque: what depends on them is made anew for each tile, not kept in registers)
-                asm volatile("" : "+s"(sa), "+s"(sb));
-                SlabA::offsets(sa, rows, off_a);
-                SlabB::offsets(sb, cols, off_b);
-                return true;
-            }
+            Tile<T> t;
+            if (!take(t)) return false;
+            A = uniform(t.a), B = uniform(t.b), C = uniform(t.c);
+            rows = __builtin_amdgcn_readfirstlane(t.rows), cols = __builtin_amdgcn_readfirstlane(t.cols), depth = __builtin_amdgcn_readfirstlane(t.depth);
+            steps = (depth + kStep<T> - 1) / kStep<T>, whole = depth / kStep<T>;
+            uint32_t sa = stride_a, sb = stride_b;// (opaque: what depends on them is made anew for each tile, not kept in registers)
+            asm volatile("" : "+s"(sa), "+s"(sb));
+            SlabA::offsets(sa, rows, off_a);
+            SlabB::offsets(sb, cols, off_b);
+            return true;
         };
         auto slot_after = [](uint32_t slot, uint32_t n) { return slot + n >= kSlots ? slot + n - kSlots : slot + n; };
         auto dst_of     = [&](uint32_t slot) { return lds0 + slot * kSlabBytes; };
@@ -417,9 +380,9 @@ namespace splahip {
             if (steps) {
                 if constexpr (LOAD == kElements) {
                     fetch_a(0), fetch_b(0);
-                    SlabA::put(ra, slabs[0]), SlabB::put(rb, slabs[1]);
+                    SlabA::put(ra, slabs(0)), SlabB::put(rb, slabs(1));
                     fetch_a(1);
-                    SlabA::put(ra, slabs[2]);
+                    SlabA::put(ra, slabs(2));
                     fetch_b(1), fetch_a(2);
                 } else {
                     // the first two slabs: behind them three more, and a whole tile's stores
@@ -433,9 +396,9 @@ namespace splahip {
                 __syncthreads();
                 s16x8 fa[2][TM], fb[2][TN];
 #pragma unroll
-                for (uint32_t j = 0; j < TN; ++j) fb[0][j] = operand<T, BN, B_DEPTH>(slabs[1], wn + j * 32, 0);
+                for (uint32_t j = 0; j < TN; ++j) fb[0][j] = operand<T, BN, B_DEPTH>(slabs(1), wn + j * 32, 0);
 #pragma unroll
-                for (uint32_t i = 0; i < TM; ++i) fa[0][i] = operand<T, BM, A_DEPTH>(slabs[0], wm + i * 32, 0);
+                for (uint32_t i = 0; i < TM; ++i) fa[0][i] = operand<T, BM, A_DEPTH>(slabs(0), wm + i * 32, 0);
                 // quarter q's matrix instructions; the next quarter's operands are read meanwhile, and with `load` the loads of B's slab ls and A's next one issued
                 auto quarter = [&](auto q_, auto load_, const T* as, const T* bs, uint32_t ls, uint32_t slot) {
                     constexpr uint32_t q = decltype(q_)::value, cur = q & 1u, k0 = (q + 1) % 4 * kQuarter;
@@ -464,11 +427,11 @@ namespace splahip {
                 constexpr integral_constant<bool, false> no{};
                 uint32_t                                 slot = 0;// of A's slab
                 auto                                     step = [&](auto load_, uint32_t s) {
-                    const T *as = slabs[slot], *bs = slabs[slot_after(slot, 1)];
+                    const T *as = slabs(slot), *bs = slabs(slot_after(slot, 1));
                     quarter(integral_constant<uint32_t, 0>{}, no, as, bs, 0, 0);
                     quarter(integral_constant<uint32_t, 1>{}, no, as, bs, 0, 0);
                     quarter(integral_constant<uint32_t, 2>{}, no, as, bs, 0, 0);
-                    if constexpr (LOAD == kElements) SlabB::put(rb, slabs[slot_after(slot, 3)]), SlabA::put(ra, slabs[slot_after(slot, 4)]);
+                    if constexpr (LOAD == kElements) SlabB::put(rb, slabs(slot_after(slot, 3))), SlabA::put(ra, slabs(slot_after(slot, 4)));
                     else if (decltype(load_)::value)
                         loads_arrived<LOADS>();
                     else
@@ -478,7 +441,7 @@ namespace splahip {
                     if constexpr (LOAD == kElements) fetch_b(s + 2), fetch_a(s + 3);
                     else if (!decltype(load_)::value)
                         slab_b(s + 2, slot), slab_a(s + 3, slot_after(slot, 1));
-                    quarter(integral_constant<uint32_t, 3>{}, load_, slabs[slot_after(slot, 2)], slabs[slot_after(slot, 3)], s + 2, slot);
+                    quarter(integral_constant<uint32_t, 3>{}, load_, slabs(slot_after(slot, 2)), slabs(slot_after(slot, 3)), s + 2, slot);
                     slot = slot_after(slot, 2);
                 };
                 uint32_t s = 0;
@@ -504,7 +467,7 @@ namespace splahip {
             };
             if constexpr (kTurns) {
                 // every wavefront turns its part in LDS and stores lines
-                T*   turn = slabs[4] + wave * (32 * kTurnCols);
+                T*   turn = slabs(4) + wave * (32 * kTurnCols);
                 auto swz  = [](uint32_t m) { return (m / (16 / kRowUnits)) % kRowUnits; };
 #pragma unroll
                 for (uint32_t i = 0; i < TM; ++i)
@@ -544,6 +507,91 @@ namespace splahip {
                             if (gm < out_rows && gn < out_cols) store_part<(BM > 128)>(out + (size_t) gm * ldc + gn, out_cols - gn, __builtin_bit_cast(s16x8, quad(i, j, v)));
                         }
             }
+        }
+    }
+
+    // SPLIT: the tiles left over when every workgroup has had the same number are cut in four, if there are few of them: most CUs would wait for a whole tile's time
+    // otherwise (132 row tiles x 16 columns on 256 CUs: nine tiles' time for 8.25 tiles' work).
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT>
+    __global__ __launch_bounds__(WM* WN * 64, OCC) void product_kernel(const ProductArgs g, uint32_t col_tiles) {
+        __shared__ __align__(1024) T lds[5 * BM * kStep<T>];
+        const uint32_t lane = threadIdx.x & 63u;
+        RowTiles       tiles{};
+        const uint32_t m_tiles = (g.m + BM - 1) / BM;// kMatrixGrad: row tiles of an expert
+        if (FORM != kMatrixGrad) tiles = row_tiles_of(BM, g.n_experts, g.n_places, g.offsets);
+        const uint32_t n_tiles = (FORM == kMatrixGrad ? g.n_experts * m_tiles : tiles.total) * col_tiles;
+        const bool     ranked = FORM == kMatrixGrad && g.n_experts <= 64;
+        uint32_t       rank = 0;
+        if (ranked && lane < g.n_experts) {
+            const uint32_t begin = bounded(g.offsets, lane, g.n_experts, g.n_places), end = bounded(g.offsets, lane + 1, g.n_experts, g.n_places);
+            rank                 = end > begin ? end - begin : 0u;
+        }
+        if (ranked) rank = rank_by_rows(rank, g.n_experts);
+
+        // The tiles go out in runs of RUN neighbours, a run to RUN workgroups of one XCD (workgroup b runs in XCD b % 8), whose L2 then holds what they share; the runs go to
+        // such groups in turn.  kForward, kRowGrad: every tile costs the same and a run fills an XCD.  kMatrixGrad: a tile's cost is its expert's number of rows;
+        // the experts go out by falling number, there and back over the groups, in shorter runs (one expert's tiles on one XCD made it the last by a third).
+        constexpr uint32_t RUN = FORM == kMatrixGrad ? 8 : 32, HIGH = FORM == kMatrixGrad ? 2 : 4;
+        auto               tile = [&](uint32_t t, Tile<T>& out) {
+            const TileAt   at = FORM == kMatrixGrad ? tile_at<HIGH>(t % (m_tiles * col_tiles), m_tiles, col_tiles) : tile_at<HIGH>(t, tiles.total, col_tiles);
+            const uint32_t n0 = at.col * BM;
+            out.cols          = min(BM, g.n - n0);
+            if (FORM == kMatrixGrad) {
+                uint32_t expert = t / (m_tiles * col_tiles);
+                if (ranked) expert = __ffsll((unsigned long long) __ballot(lane < g.n_experts && rank == expert)) - 1;
+                const uint32_t m0 = at.row * BM;
+                const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
+                out.rows             = min(BM, g.m - m0);
+                out.depth            = end > begin ? end - begin : 0u;
+                out.a = static_cast<const T*>(g.a) + (size_t) begin * g.m + m0;
+                out.b = static_cast<const T*>(g.b) + (size_t) begin * g.n + n0;
+                out.c = static_cast<T*>(g.c) + ((size_t) expert * g.m + m0) * g.n + n0;
+            } else {
+                const RowTile  r = row_tile(tiles, at.row, BM, g.n_experts, g.n_places, g.offsets);
+                const uint32_t e = min(r.expert, g.n_experts - 1);
+                out.rows         = r.rows;
+                out.depth        = r.expert < g.n_experts ? g.k : 0u;
+                out.a = static_cast<const T*>(g.a) + (size_t) r.row0 * g.k;
+                out.b = static_cast<const T*>(g.b) + (FORM == kForward ? ((size_t) e * g.n + n0) * g.k : (size_t) e * g.n * g.k + n0);
+                out.c = static_cast<T*>(g.c) + (size_t) r.row0 * g.n + n0;
+            }
+        };
+        const uint32_t groups = gridDim.x / RUN, group = blockIdx.x / 8 / RUN * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % RUN;// (the grid is a multiple of 8 RUN)
+        uint32_t       left = n_tiles % gridDim.x;
+        if (!SPLIT || left * 2 > gridDim.x) left = 0;
+        const uint32_t n_whole = n_tiles - left;
+        uint32_t       round = 0;
+        run_tiles<T, FORM, LOAD, BM, WM, WN>(g, lds, [&](Tile<T>& out) {
+            for (;; ++round) {
+                const uint64_t run = (uint64_t) round * groups + (FORM == kMatrixGrad && (round & 1u) ? groups - 1 - group : group);
+                if ((uint64_t) round * groups * RUN >= n_whole) return false;
+                if (run * RUN + in >= n_whole) continue;
+                tile((uint32_t) run * RUN + in, out);
+                ++round;
+                return true;
+            }
+        });
+        if constexpr (SPLIT) {
+            if (left == 0) return;
+            __syncthreads();// the slabs' memory changes hands
+            constexpr uint32_t HALF = BM / 2, WAVES = WM * WN;
+            // four neighbouring parts per tile, a contiguous stretch of them per XCD
+            const uint32_t parts = left * 4, per = (parts + 7) / 8, end = min(parts, (blockIdx.x % 8 + 1) * per);
+            uint32_t       part = blockIdx.x % 8 * per + blockIdx.x / 8;
+            run_tiles<T, FORM, LOAD, HALF, 2, WAVES / 2>(g, lds, [&](Tile<T>& out) {
+                for (; part < end; part += gridDim.x / 8) {
+                    tile(n_whole + part / 4, out);
+                    const uint32_t r = part % 4 / 2 * HALF, c = part % 2 * HALF;
+                    if (r >= out.rows || c >= out.cols) continue;
+                    out.rows = min(HALF, out.rows - r), out.cols = min(HALF, out.cols - c);
+                    out.a += FORM == kMatrixGrad ? r : (size_t) r * g.k;
+                    out.b += FORM == kForward ? (size_t) c * g.k : c;
+                    out.c += (size_t) r * g.n + c;
+                    part += gridDim.x / 8;
+                    return true;
+                }
+                return false;
+            });
         }
     }
 
@@ -656,13 +704,13 @@ namespace splahip {
         return SPLAHIP_OK;
     }
 
-    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC>
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT = false>
     static int launch_tiles(const ProductArgs& g, hipStream_t s) {
         const uint64_t col_tiles = (g.n + BM - 1) / BM;
         const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + BM - 1) / BM) : row_tiles_bound(g.n_places, g.n_experts, BM);
         SPLAHIP_REQUIRE(col_tiles * row_tiles < (1ull << 31), "too many tiles for one launch");
         constexpr uint32_t kResident = 256 * (OCC * 4 / (WM * WN));// workgroups the card holds at once
-        product_kernel<T, FORM, LOAD, BM, WM, WN, OCC><<<kResident, WM * WN * 64, 0, s>>>(g, (uint32_t) col_tiles);
+        product_kernel<T, FORM, LOAD, BM, WM, WN, OCC, SPLIT><<<kResident, WM * WN * 64, 0, s>>>(g, (uint32_t) col_tiles);
         SPLAHIP_TRY(hipGetLastError());
         return SPLAHIP_OK;
     }
@@ -677,11 +725,11 @@ namespace splahip {
                 return min(g.n_places, g.n_experts) * (uint64_t) (g.n / 64) >= 1024 ? launch_few_rows<T, 4>(g, s) : launch_few_rows<T, 2>(g, s);
         if constexpr (sizeof(T) == 4) {
             const bool large = tiles(128) >= 400;
-            if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);
-            return large ? launch_tiles<T, FORM, kWords, 128, 2, 2, 2>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
+            if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);
+            return large ? launch_tiles<T, FORM, kWords, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
         } else {
             if (!aligned) return launch_tiles<T, FORM, kElements, 128, 2, 2, 2>(g, s);
-            return tiles(256) >= 200 ? launch_tiles<T, FORM, kUnits, 256, 2, 4, 2>(g, s) : launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s);
+            return tiles(256) >= 200 ? launch_tiles<T, FORM, kUnits, 256, 2, 4, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s);
         }
     }
 

@@ -204,11 +204,12 @@ def test_product_of_any_numbers(rows, k, experts, n_in, n_out, dtype):
     _close(got_dw, dw, sdw * (rows * k * 2 * U), dtype)
 
 
-# enough tiles that the card is full of large ones: ragged ranges, depths that end inside a slab, experts without rows, more experts than a wavefront has lanes
-LARGE = [(6000, 2, 5, 328, 2056), (2600, 2, 70, 136, 2304), (700, 1, 200, 264, 520), (9000, 1, 2, 64, 2048), (3000, 2, 3, 2120, 1288)]
+# enough tiles that the card is full of large ones, with some left over that are cut in parts: ragged ranges, depths that end inside a slab, experts without rows, more experts than a wavefront has lanes
+LARGE = [(6000, 2, 5, 328, 2056), (2600, 2, 70, 136, 2304), (700, 1, 200, 264, 520), (9000, 1, 2, 64, 2048), (3000, 2, 3, 2120, 1288), (4800, 2, 2, 2048, 264),
+         (6000, 2, 3, 516, 768), (6000, 2, 3, 515, 769), (3000, 2, 20, 515, 769), (2600, 2, 30, 776, 1288)]
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,k,experts,n_in,n_out", LARGE)
 def test_large_products_of_whole_numbers(rows, k, experts, n_in, n_out, dtype):
     """sums below 2^24 are exact in fp32 (and in the reference's fp32 product); values -1, 0, 1 keep fp16 results below its largest value"""
