@@ -427,13 +427,15 @@ int splahip_route_back_grad(int panel_type, uint32_t n_rows, uint32_t per_row, u
                             const float* d_weights, const void* d_y, const void* d_dout, void* d_dy, float* d_dweights, void* stream);
 /* expert_product: with the rows in expert order, d_y[p, :] = d_w[e] d_x[p, :] for p in [d_offsets[e], d_offsets[e + 1]), d_w = [n_experts, n_out, n_in] row-major; the
  * rows behind the last entry become 0 and are not read.  _dx: d_dx[p, :] = d_w[e]^T d_dy[p, :].  _dw: d_dw[e] = sum of d_dy[p, :] d_x[p, :]^T over the expert's
- * rows (0 without rows).  fp32 panels are multiplied in full fp32. */
+ * rows (0 without rows); its workspace (16-byte aligned) takes the sums of parts of the rows where the matrices are too small to fill the card by themselves.
+ * fp32 panels are multiplied in full fp32.  n_in, n_out < 2^21. */
 int splahip_expert_product(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_x,
                            const void* d_w, void* d_y, void* stream);
 int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_dy,
                               const void* d_w, void* d_dx, void* stream);
+size_t splahip_expert_product_dw_workspace(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out); /* bytes, often 0 */
 int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_dy,
-                              const void* d_x, void* d_dw, void* stream);
+                              const void* d_x, void* d_dw, void* d_workspace, size_t workspace_bytes, void* stream);
 /* global_norm: *d_norm = sqrt of the sum of the squares of all elements of all arrays (h_ lists on the host: addresses, lengths in elements, panel types); squares
  * and sums in 64 bits.  clip_global_norm: h_out[i] = h_arrays[i] * min(1, limit / norm) (h_out[i] may be h_arrays[i]; no other overlap); a norm that is not
  * finite scales nothing.  norm_given != 0: *d_norm is the norm to use (of arrays on several devices, say) and is read; else it is computed and written.

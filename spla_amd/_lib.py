@@ -133,13 +133,14 @@ _SIGNATURES = {
     "splahip_route_back_grad": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "splahip_expert_product": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
     "splahip_expert_product_dx": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
-    "splahip_expert_product_dw": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
+    "splahip_expert_product_dw_workspace": (C.c_size_t, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
+    "splahip_expert_product_dw": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "splahip_global_norm_workspace": (C.c_size_t, [C.c_uint32, _vp]),
     "splahip_global_norm": (C.c_int, [C.c_uint32, _vp, _vp, _vp, _vp, C.c_size_t, _vp, _vp]),
     "splahip_clip_global_norm": (C.c_int, [C.c_uint32, _vp, _vp, _vp, _vp, C.c_float, C.c_int, _vp, C.c_size_t, _vp, _vp]),
 }
 _RAW = {"splahip_set_deterministic", "splahip_set_reference_order", "splahip_mxv_prefers_sell", "splahip_device_count", "splahip_last_error", "splahip_version", "splahip_mxv_variant", "splahip_mxv_variant_of", "splahip_dist_available",
-        "splahip_route_sort_workspace", "splahip_global_norm_workspace", "splahip_shard_split_serves", "splahip_shard_prefers_whole", "splahip_jit_available"}
+        "splahip_route_sort_workspace", "splahip_expert_product_dw_workspace", "splahip_global_norm_workspace", "splahip_shard_split_serves", "splahip_shard_prefers_whole", "splahip_jit_available"}
 
 _lib = None
 

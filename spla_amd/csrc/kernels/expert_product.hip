@@ -8,6 +8,7 @@
 // Rows behind the last entry (offsets[n_experts] ..) become 0; an expert without rows has dw = 0.  fp32 sums in a fixed order, one rounding to the panel's
 // type.  fp32 panels are multiplied in full fp32 (v_mfma_f32_32x32x2_f32).
 #include "panel.hpp"
+#include <algorithm>
 #include <type_traits>
 
 
@@ -131,6 +132,7 @@ namespace splahip {
         void*       c;
         uint32_t    n_places, n_experts, m, n, k;// kForward: n = n_out, k = n_in; kRowGrad: n = n_in, k = n_out; kMatrixGrad: m = n_out, n = n_in
         const uint32_t* offsets;
+        uint32_t        splits = 1;// kMatrixGrad: parts that an expert's rows are taken in, c then = fp32 [splits, n_experts, m, n]
     };
 
     // ---- LDS ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -300,15 +302,15 @@ namespace splahip {
         }
     }
 
-    template<typename T>
+    template<typename T, typename O>
     struct Tile {
         const T *a, *b;
-        T*       c;
+        O*       c;
         uint32_t rows, cols, depth;
     };
 
-    // take(tile): the workgroup's next tile, false behind the last
-    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, typename TAKE>
+    // take(tile): the workgroup's next tile, false behind the last.  O: the result's type, T or (partial sums) float
+    template<typename T, typename O, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, typename TAKE>
     __device__ __forceinline__ void run_tiles(const ProductArgs& g, T* lds, TAKE&& take) {
         constexpr uint32_t BN = BM, THREADS = WM * WN * 64, TM = BM / WM / 32, TN = BN / WN / 32;
         constexpr bool     A_DEPTH = FORM != kMatrixGrad, B_DEPTH = FORM == kForward;
@@ -319,7 +321,7 @@ namespace splahip {
         constexpr uint32_t kMul       = TM * TN, kReads = TM + TN, kReadsPer = (kReads + kMul - 1) / kMul, kQuarter = 2 * kUnit<T>;
         // the result is turned in the fifth slab, 32 rows x kTurn tiles of 32 columns at a time and wavefront
         constexpr uint32_t kTurn = sizeof(T) == 2 ? TN : 1, kTurnCols = kTurn * 32, kRowUnits = kTurnCols / kUnit<T>;
-        constexpr bool     kTurns = WM * WN * 32 * kTurnCols <= kSlab;
+        constexpr bool     kTurns = std::is_same_v<T, O> && WM * WN * 32 * kTurnCols <= kSlab;
         constexpr uint32_t kStores = kTurns ? TM * (TN / kTurn) * 32 * kRowUnits / 64 : TM * TN * 4;
         auto slabs = [&](uint32_t slot) { return lds + slot * kSlab; };
         const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -331,11 +333,11 @@ namespace splahip {
 
         // the tile at hand
         const T *A, *B;
-        T*       C;
+        O*       C;
         uint32_t rows, cols, depth, steps, whole;
         uint32_t off_a[LOADS], off_b[LOADS];
         auto     next = [&]() -> bool {
-            Tile<T> t;
+            Tile<T, O> t;
             if (!take(t)) return false;
             A = uniform(t.a), B = uniform(t.b), C = uniform(t.c);
             rows = __builtin_amdgcn_readfirstlane(t.rows), cols = __builtin_amdgcn_readfirstlane(t.cols), depth = __builtin_amdgcn_readfirstlane(t.depth);
@@ -450,7 +452,7 @@ namespace splahip {
                 for (; s < steps; ++s) step(no, s);
                 __syncthreads();// nothing reads a slab any more
             }
-            T* const       out = C;
+            O* const       out = C;
             uint32_t       ldc = g.n;
             asm volatile("" : "+s"(ldc));
             const uint32_t out_rows = rows, out_cols = cols;
@@ -459,10 +461,10 @@ namespace splahip {
             stored = out_rows == BM && out_cols == BN;
             // A lane holds four neighbouring columns of a row, its neighbours hold other rows.
             auto quad = [&](uint32_t i, uint32_t j, uint32_t v) {
-                typedef T four __attribute__((ext_vector_type(4)));
+                typedef O four __attribute__((ext_vector_type(4)));
                 four      c;
 #pragma unroll
-                for (uint32_t q = 0; q < 4; ++q) c[q] = (T) acc[i][j][v + q];
+                for (uint32_t q = 0; q < 4; ++q) c[q] = (O) acc[i][j][v + q];
                 return c;
             };
             if constexpr (kTurns) {
@@ -512,14 +514,15 @@ namespace splahip {
 
     // SPLIT: the tiles left over when every workgroup has had the same number are cut in four, if there are few of them: most CUs would wait for a whole tile's time
     // otherwise (132 row tiles x 16 columns on 256 CUs: nine tiles' time for 8.25 tiles' work).
-    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT>
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT, bool PARTIAL>
     __global__ __launch_bounds__(WM* WN * 64, OCC) void product_kernel(const ProductArgs g, uint32_t col_tiles) {
         __shared__ __align__(1024) T lds[5 * BM * kStep<T>];
         const uint32_t lane = threadIdx.x & 63u;
         RowTiles       tiles{};
         const uint32_t m_tiles = (g.m + BM - 1) / BM;// kMatrixGrad: row tiles of an expert
         if (FORM != kMatrixGrad) tiles = row_tiles_of(BM, g.n_experts, g.n_places, g.offsets);
-        const uint32_t n_tiles = (FORM == kMatrixGrad ? g.n_experts * m_tiles : tiles.total) * col_tiles;
+        using O                = std::conditional_t<PARTIAL, float, T>;
+        const uint32_t n_tiles = (FORM == kMatrixGrad ? g.n_experts * m_tiles * (PARTIAL ? g.splits : 1u) : tiles.total) * col_tiles;
         const bool     ranked = FORM == kMatrixGrad && g.n_experts <= 64;
         uint32_t       rank = 0;
         if (ranked && lane < g.n_experts) {
@@ -532,20 +535,27 @@ namespace splahip {
         // such groups in turn.  kForward, kRowGrad: every tile costs the same and a run fills an XCD.  kMatrixGrad: a tile's cost is its expert's number of rows;
         // the experts go out by falling number, there and back over the groups, in shorter runs (one expert's tiles on one XCD made it the last by a third).
         constexpr uint32_t RUN = FORM == kMatrixGrad ? 8 : 32, HIGH = FORM == kMatrixGrad ? 2 : 4;
-        auto               tile = [&](uint32_t t, Tile<T>& out) {
-            const TileAt   at = FORM == kMatrixGrad ? tile_at<HIGH>(t % (m_tiles * col_tiles), m_tiles, col_tiles) : tile_at<HIGH>(t, tiles.total, col_tiles);
+        auto               tile = [&](uint32_t t, Tile<T, O>& out) {
+            const uint32_t each = m_tiles * col_tiles, part = PARTIAL ? t / each % g.splits : 0u;// tiles of an expert and part, the part
+            const TileAt   at = FORM == kMatrixGrad ? tile_at<HIGH>(t % each, m_tiles, col_tiles) : tile_at<HIGH>(t, tiles.total, col_tiles);
             const uint32_t n0 = at.col * BM;
             out.cols          = min(BM, g.n - n0);
             if (FORM == kMatrixGrad) {
-                uint32_t expert = t / (m_tiles * col_tiles);
+                uint32_t expert = t / (each * (PARTIAL ? g.splits : 1u));
                 if (ranked) expert = __ffsll((unsigned long long) __ballot(lane < g.n_experts && rank == expert)) - 1;
                 const uint32_t m0 = at.row * BM;
-                const uint32_t begin = bounded(g.offsets, expert, g.n_experts, g.n_places), end = bounded(g.offsets, expert + 1, g.n_experts, g.n_places);
-                out.rows             = min(BM, g.m - m0);
-                out.depth            = end > begin ? end - begin : 0u;
+                uint32_t       begin = bounded(g.offsets, expert, g.n_experts, g.n_places);
+                const uint32_t end = max(begin, bounded(g.offsets, expert + 1, g.n_experts, g.n_places));
+                out.rows           = min(BM, g.m - m0);
+                out.depth          = end - begin;
+                if (PARTIAL) {// whole steps to each part
+                    const uint32_t chunk = ((out.depth + kStep<T> - 1) / kStep<T> + g.splits - 1) / g.splits * kStep<T>;
+                    begin                = min(begin + part * chunk, end);
+                    out.depth            = min(chunk, end - begin);
+                }
                 out.a = static_cast<const T*>(g.a) + (size_t) begin * g.m + m0;
                 out.b = static_cast<const T*>(g.b) + (size_t) begin * g.n + n0;
-                out.c = static_cast<T*>(g.c) + ((size_t) expert * g.m + m0) * g.n + n0;
+                out.c = static_cast<O*>(g.c) + (((size_t) part * g.n_experts + expert) * g.m + m0) * g.n + n0;
             } else {
                 const RowTile  r = row_tile(tiles, at.row, BM, g.n_experts, g.n_places, g.offsets);
                 const uint32_t e = min(r.expert, g.n_experts - 1);
@@ -553,7 +563,7 @@ namespace splahip {
                 out.depth        = r.expert < g.n_experts ? g.k : 0u;
                 out.a = static_cast<const T*>(g.a) + (size_t) r.row0 * g.k;
                 out.b = static_cast<const T*>(g.b) + (FORM == kForward ? ((size_t) e * g.n + n0) * g.k : (size_t) e * g.n * g.k + n0);
-                out.c = static_cast<T*>(g.c) + (size_t) r.row0 * g.n + n0;
+                out.c = static_cast<O*>(g.c) + (size_t) r.row0 * g.n + n0;
             }
         };
         const uint32_t groups = gridDim.x / RUN, group = blockIdx.x / 8 / RUN * 8 + blockIdx.x % 8, in = blockIdx.x / 8 % RUN;// (the grid is a multiple of 8 RUN)
@@ -561,7 +571,7 @@ namespace splahip {
         if (!SPLIT || left * 2 > gridDim.x) left = 0;
         const uint32_t n_whole = n_tiles - left;
         uint32_t       round = 0;
-        run_tiles<T, FORM, LOAD, BM, WM, WN>(g, lds, [&](Tile<T>& out) {
+        run_tiles<T, O, FORM, LOAD, BM, WM, WN>(g, lds, [&](Tile<T, O>& out) {
             for (;; ++round) {
                 const uint64_t run = (uint64_t) round * groups + (FORM == kMatrixGrad && (round & 1u) ? groups - 1 - group : group);
                 if ((uint64_t) round * groups * RUN >= n_whole) return false;
@@ -578,7 +588,7 @@ namespace splahip {
             // four neighbouring parts per tile, a contiguous stretch of them per XCD
             const uint32_t parts = left * 4, per = (parts + 7) / 8, end = min(parts, (blockIdx.x % 8 + 1) * per);
             uint32_t       part = blockIdx.x % 8 * per + blockIdx.x / 8;
-            run_tiles<T, FORM, LOAD, HALF, 2, WAVES / 2>(g, lds, [&](Tile<T>& out) {
+            run_tiles<T, O, FORM, LOAD, HALF, 2, WAVES / 2>(g, lds, [&](Tile<T, O>& out) {
                 for (; part < end; part += gridDim.x / 8) {
                     tile(n_whole + part / 4, out);
                     const uint32_t r = part % 4 / 2 * HALF, c = part % 2 * HALF;
@@ -704,32 +714,81 @@ namespace splahip {
         return SPLAHIP_OK;
     }
 
-    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT = false>
+    // out = the sum of the parts, in their order
+    template<typename T>
+    __global__ __launch_bounds__(256) void join_parts_kernel(uint64_t n, uint32_t parts, const float* __restrict__ part, T* __restrict__ out) {
+        for (uint64_t i = (uint64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t) gridDim.x * 256) {
+            float s = 0.0f;
+#pragma unroll 8
+            for (uint32_t p = 0; p < parts; ++p) s += part[p * n + i];
+            out[i] = (T) s;
+        }
+    }
+
+    template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT = false, bool PARTIAL = false>
     static int launch_tiles(const ProductArgs& g, hipStream_t s) {
         const uint64_t col_tiles = (g.n + BM - 1) / BM;
-        const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * ((g.m + BM - 1) / BM) : row_tiles_bound(g.n_places, g.n_experts, BM);
+        const uint64_t row_tiles = FORM == kMatrixGrad ? (uint64_t) g.n_experts * g.splits * ((g.m + BM - 1) / BM) : row_tiles_bound(g.n_places, g.n_experts, BM);
         SPLAHIP_REQUIRE(col_tiles * row_tiles < (1ull << 31), "too many tiles for one launch");
         constexpr uint32_t kResident = 256 * (OCC * 4 / (WM * WN));// workgroups the card holds at once
-        product_kernel<T, FORM, LOAD, BM, WM, WN, OCC, SPLIT><<<kResident, WM * WN * 64, 0, s>>>(g, (uint32_t) col_tiles);
+        product_kernel<T, FORM, LOAD, BM, WM, WN, OCC, SPLIT, PARTIAL><<<kResident, WM * WN * 64, 0, s>>>(g, (uint32_t) col_tiles);
         SPLAHIP_TRY(hipGetLastError());
         return SPLAHIP_OK;
     }
 
+    static uint64_t matrix_tiles(const ProductArgs& g, uint64_t bm) { return g.n_experts * ((g.m + bm - 1) / bm) * ((g.n + bm - 1) / bm); }
+    // the size of tile that fills the card
+    static uint32_t matrix_grad_tile(const ProductArgs& g, uint32_t element, bool aligned) {
+        if (element == 4) return matrix_tiles(g, 128) >= 400 ? 128 : 64;
+        return aligned && matrix_tiles(g, 256) >= 200 ? 256 : 128;
+    }
+    // kMatrixGrad: parts that the experts' rows are taken in where there are too few tiles to fill the card: up to about 512 tiles in all, six steps of k or more for each on
+    // the average, and no more parts than pay: S parts save (1 - 1/S) of the steps (t = 0.9 us each in fp32, 0.4 in 16 bits) and write and read S N fp32 sums
+    // (5 TB/s), least at S^2 = steps t 5 TB/s / 8 N.  (The gradient for 5 matrices of 250 x 333 over 4800 fp32 rows, 120 tiles of 30 steps: 27 us in one part, 20 in four.)
+    static uint32_t matrix_grad_splits(const ProductArgs& g, uint32_t element, bool aligned) {
+        const uint32_t bm = matrix_grad_tile(g, element, aligned);
+        if (bm == 256) return 1;
+        const uint64_t steps = g.n_places / g.n_experts / (128 / element), most = std::min<uint64_t>({512 / std::max<uint64_t>(matrix_tiles(g, bm), 1), steps / 6, 16});
+        const uint64_t n     = (uint64_t) g.n_experts * g.m * g.n;
+        uint32_t       parts = 1;
+        while (parts < most && (uint64_t) (parts + 1) * (parts + 1) * n <= steps * (element == 4 ? 562500 : 250000)) ++parts;
+        return parts;
+    }
+
+    static bool aligned_product(const ProductArgs& g, uint32_t unit) {
+        return ((uintptr_t) g.a % 16 == 0) && ((uintptr_t) g.b % 16 == 0) && ((uintptr_t) g.c % 16 == 0) && g.n % unit == 0 && g.k % unit == 0 && g.m % unit == 0;
+    }
+
     template<Form FORM, typename T>
     static int launch_of_type(const ProductArgs& g, hipStream_t s) {
-        const uint32_t u       = kUnit<T>;
-        const bool     aligned = ((uintptr_t) g.a % 16 == 0) && ((uintptr_t) g.b % 16 == 0) && ((uintptr_t) g.c % 16 == 0) && g.n % u == 0 && g.k % u == 0 && g.m % u == 0;
-        auto tiles = [&](uint64_t bm) { return (FORM == kMatrixGrad ? g.n_experts * ((g.m + bm - 1) / bm) : g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
-        if constexpr (FORM == kForward)
-            if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts)
-                return min(g.n_places, g.n_experts) * (uint64_t) (g.n / 64) >= 1024 ? launch_few_rows<T, 4>(g, s) : launch_few_rows<T, 2>(g, s);
-        if constexpr (sizeof(T) == 4) {
-            const bool large = tiles(128) >= 400;
-            if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);
-            return large ? launch_tiles<T, FORM, kWords, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
+        const bool aligned = aligned_product(g, kUnit<T>);
+        if constexpr (FORM == kMatrixGrad) {
+            const uint32_t bm = matrix_grad_tile(g, sizeof(T), aligned);
+            if constexpr (sizeof(T) == 4) {
+                if (g.splits > 1) {
+                    if (bm == 128) return aligned ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, false, true>(g, s) : launch_tiles<T, FORM, kWords, 128, 2, 2, 2, false, true>(g, s);
+                    return aligned ? launch_tiles<T, FORM, kUnits, 64, 2, 2, 4, false, true>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4, false, true>(g, s);
+                }
+                if (bm == 128) return aligned ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kWords, 128, 2, 2, 2, true>(g, s);
+                return aligned ? launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
+            } else {
+                if (g.splits > 1) return aligned ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, false, true>(g, s) : launch_tiles<T, FORM, kElements, 128, 2, 2, 2, false, true>(g, s);
+                if (!aligned) return launch_tiles<T, FORM, kElements, 128, 2, 2, 2>(g, s);
+                return bm == 256 ? launch_tiles<T, FORM, kUnits, 256, 2, 4, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s);
+            }
         } else {
-            if (!aligned) return launch_tiles<T, FORM, kElements, 128, 2, 2, 2>(g, s);
-            return tiles(256) >= 200 ? launch_tiles<T, FORM, kUnits, 256, 2, 4, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s);
+            auto tiles = [&](uint64_t bm) { return (g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
+            if constexpr (FORM == kForward)
+                if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts)
+                    return std::min(g.n_places, g.n_experts) * (uint64_t) (g.n / 64) >= 1024 ? launch_few_rows<T, 4>(g, s) : launch_few_rows<T, 2>(g, s);
+            if constexpr (sizeof(T) == 4) {
+                const bool large = tiles(128) >= 400;
+                if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);
+                return large ? launch_tiles<T, FORM, kWords, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
+            } else {
+                if (!aligned) return launch_tiles<T, FORM, kElements, 128, 2, 2, 2>(g, s);
+                return tiles(256) >= 200 ? launch_tiles<T, FORM, kUnits, 256, 2, 4, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 128, 2, 2, 2>(g, s);
+            }
         }
     }
 
@@ -762,10 +821,35 @@ extern "C" int splahip_expert_product_dx(int panel_type, uint32_t n_places, uint
     return launch_product<kRowGrad>(panel_type, ProductArgs{d_dy, d_w, d_dx, n_places, n_experts, 0, n_in, n_out, d_offsets}, as_stream(stream));
 }
 
+// the parts' sums; 0: the call needs none
+extern "C" size_t splahip_expert_product_dw_workspace(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out) {
+    if (check_product(panel_type, n_places, n_experts, n_in, n_out)) return 0;
+    const uint32_t    element = panel_type == SPLAHIP_PANEL_FLOAT ? 4 : 2;
+    const ProductArgs g{nullptr, nullptr, nullptr, n_places, n_experts, n_out, n_in, 0, nullptr};
+    // (enough for operands of any alignment)
+    const uint32_t splits = std::max(matrix_grad_splits(g, element, true), matrix_grad_splits(g, element, false));
+    return splits > 1 ? (size_t) splits * n_experts * n_in * n_out * sizeof(float) : 0;
+}
+
 extern "C" int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets,
-                                         const void* d_dy, const void* d_x, void* d_dw, void* stream) {
+                                         const void* d_dy, const void* d_x, void* d_dw, void* d_workspace, size_t workspace_bytes, void* stream) {
     if (int st = check_product(panel_type, n_places, n_experts, n_in, n_out)) return st;
     SPLAHIP_REQUIRE(d_offsets && d_dw && (n_places == 0 || (d_dy && d_x)), "null array");
+    const size_t need = splahip_expert_product_dw_workspace(panel_type, n_places, n_experts, n_in, n_out);
+    SPLAHIP_REQUIRE(workspace_bytes >= need && (need == 0 || (d_workspace && (uintptr_t) d_workspace % 16 == 0)), "workspace too small");
     if (int st = ensure_device()) return st;
-    return launch_product<kMatrixGrad>(panel_type, ProductArgs{d_dy, d_x, d_dw, n_places, n_experts, n_out, n_in, 0, d_offsets}, as_stream(stream));
+    hipStream_t    s       = as_stream(stream);
+    const uint32_t element = panel_type == SPLAHIP_PANEL_FLOAT ? 4 : 2;
+    ProductArgs    g{d_dy, d_x, d_dw, n_places, n_experts, n_out, n_in, 0, d_offsets};
+    g.splits = matrix_grad_splits(g, element, aligned_product(g, 16 / element));
+    if (g.splits == 1) return launch_product<kMatrixGrad>(panel_type, g, s);
+    g.c = d_workspace;// (its alignment does not choose another kernel: the parts are fp32 and stored as such)
+    if (int st = launch_product<kMatrixGrad>(panel_type, g, s)) return st;
+    const uint64_t n = (uint64_t) n_experts * n_in * n_out;
+    panel_dispatch(panel_type, [&](auto zero) {
+        using T = decltype(zero);
+        join_parts_kernel<T><<<(uint32_t) std::min<uint64_t>((n + 255) / 256, 4096), 256, 0, s>>>(n, g.splits, static_cast<const float*>(d_workspace), static_cast<T*>(d_dw));
+    });
+    SPLAHIP_TRY(hipGetLastError());
+    return SPLAHIP_OK;
 }

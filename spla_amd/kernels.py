@@ -413,7 +413,9 @@ def expert_product_grad(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor, dy: t
         _launch(plan.device, "splahip_expert_product_dx", *args, offsets, src_dy, src_w, dx.data_ptr())
     if need[1]:
         dw = torch.empty_like(w)
-        _launch(plan.device, "splahip_expert_product_dw", *args, offsets, src_dy, src, dw.data_ptr())
+        n_bytes = _lib.load().splahip_expert_product_dw_workspace(*args)
+        work = torch.empty(n_bytes, dtype=torch.uint8, device=plan.device) if n_bytes else None
+        _launch(plan.device, "splahip_expert_product_dw", *args, offsets, src_dy, src, dw.data_ptr(), work.data_ptr() if n_bytes else None, n_bytes)
     return dx, dw
 
 

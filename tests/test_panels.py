@@ -79,13 +79,17 @@ def test_c_entries_refuse():
     _fails("splahip_route_rows", 0, 4, 2, 3, 1 << 30, p, p, None, p, p, None)  # width
     _fails("splahip_route_back", 0, 4, 2, 8, p, None, None, p, None)          # null
     _fails("splahip_route_back_grad", 0, 4, 2, 3, 8, p, p, None, p, p, p, p, None)  # no weights
-    for name in ("splahip_expert_product", "splahip_expert_product_dx", "splahip_expert_product_dw"):
-        _fails(name, 7, 8, 3, 4, 4, p, p, p, p, None)
-        _fails(name, 0, 8, 0, 4, 4, p, p, p, p, None)
-        _fails(name, 0, 8, 3, 0, 4, p, p, p, p, None)
-        _fails(name, 0, 8, 3, 4, 1 << 21, p, p, p, p, None)
-        _fails(name, 0, 8, 3, 4, 4, None, p, p, p, None)
-        _fails(name, 0, 1 << 31, 3, 4, 4, p, p, p, p, None)
+    for name, more in (("splahip_expert_product", ()), ("splahip_expert_product_dx", ()), ("splahip_expert_product_dw", (p, big))):
+        _fails(name, 7, 8, 3, 4, 4, p, p, p, p, *more, None)
+        _fails(name, 0, 8, 0, 4, 4, p, p, p, p, *more, None)
+        _fails(name, 0, 8, 3, 0, 4, p, p, p, p, *more, None)
+        _fails(name, 0, 8, 3, 4, 1 << 21, p, p, p, p, *more, None)
+        _fails(name, 0, 8, 3, 4, 4, None, p, p, p, *more, None)
+        _fails(name, 0, 1 << 31, 3, 4, 4, p, p, p, p, *more, None)
+    need = _lib.call("splahip_expert_product_dw_workspace", 0, 20000, 2, 40, 56)
+    assert need >= 2 * 2 * 40 * 56 * 4
+    _fails("splahip_expert_product_dw", 0, 20000, 2, 40, 56, p, p, p, p, p, need - 1, None)
+    _fails("splahip_expert_product_dw", 0, 20000, 2, 40, 56, p, p, p, p, None, need, None)
 
 
 def test_clip_refuses_overlaps_and_limits():
