@@ -779,7 +779,7 @@ namespace splahip {
         } else {
             auto tiles = [&](uint64_t bm) { return (g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
             if constexpr (FORM == kForward)
-                if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts)
+                if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts && g.n_experts * (uint64_t) (g.n / 32 + 1) < (1u << 23))// (a launch holds fewer than 2^32 threads)
                     return std::min(g.n_places, g.n_experts) * (uint64_t) (g.n / 64) >= 1024 ? launch_few_rows<T, 4>(g, s) : launch_few_rows<T, 2>(g, s);
             if constexpr (sizeof(T) == 4) {
                 const bool large = tiles(128) >= 400;

@@ -217,7 +217,7 @@ namespace splahip {
 
     // no two results may share memory, and a result may share it with its own source only, element for element: anything else would be scaled twice or read
     // after it was scaled
-    static int check_overlap(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types) {
+    static int check_overlap(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types, const float* norm) {
         struct Span {
             uintptr_t a, b;
             uint32_t  i;
@@ -229,11 +229,15 @@ namespace splahip {
             if (lengths[i]) out.push_back(span(dst[i], i));
         std::sort(out.begin(), out.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
         for (size_t k = 1; k < out.size(); ++k) SPLAHIP_REQUIRE(out[k - 1].b <= out[k].a, "results overlap (the same array twice?)");
+        auto free_of_results = [&](uintptr_t a, uintptr_t b) {
+            auto it = std::upper_bound(out.begin(), out.end(), a, [](uintptr_t p, const Span& y) { return p < y.b; });
+            return it == out.end() || it->a >= b;
+        };
+        SPLAHIP_REQUIRE(free_of_results((uintptr_t) norm, (uintptr_t) norm + sizeof(float)), "the norm lies inside a result");
         for (uint32_t i = 0; i < n_arrays; ++i) {
             if (lengths[i] == 0 || src[i] == dst[i]) continue;// (its own result: the check above covers the others)
-            const Span x  = span(src[i], i);
-            auto       it = std::upper_bound(out.begin(), out.end(), x.a, [](uintptr_t a, const Span& y) { return a < y.b; });
-            SPLAHIP_REQUIRE(it == out.end() || it->a >= x.b, "an array overlaps a result other than itself");
+            const Span x = span(src[i], i);
+            SPLAHIP_REQUIRE(free_of_results(x.a, x.b), "an array overlaps a result other than itself");
         }
         return SPLAHIP_OK;
     }
@@ -277,7 +281,7 @@ extern "C" int splahip_clip_global_norm(uint32_t n_arrays, const void* const* h_
     SPLAHIP_REQUIRE(n_arrays == 0 || h_out, "null list");
     for (uint32_t i = 0; i < n_arrays; ++i) SPLAHIP_REQUIRE(h_lengths[i] == 0 || h_out[i], "null array");
     try {
-        if (int st = check_overlap(n_arrays, h_arrays, h_out, h_lengths, h_types)) return st;
+        if (int st = check_overlap(n_arrays, h_arrays, h_out, h_lengths, h_types, d_norm)) return st;
     } catch (const std::bad_alloc&) { return fail(SPLAHIP_ERROR, "out of host memory"); }
     if (!norm_given)
         if (int st = splahip_global_norm(n_arrays, h_arrays, h_lengths, h_types, d_workspace, workspace_bytes, d_norm, stream)) return st;

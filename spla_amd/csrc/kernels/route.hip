@@ -11,6 +11,7 @@
 // Every sum has a fixed order: results are the same from run to run.
 #include "panel.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace splahip {
@@ -292,17 +293,16 @@ namespace splahip {
             clear_rows(out, min(offsets[n_experts], n_places), n_places, width, blockIdx.x - row_blocks, gridDim.x - row_blocks, shift);
             return;
         }
-        const uint32_t r = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
-        if (r >= n_rows) return;
-        for (uint32_t c = sub * U; c < width; c += lanes * U) {
-            const auto v = unit_at<T, LARGE>(x + (size_t) r * width + c, width - c);
-            for (uint32_t j = 0; j < per_row; ++j) {
-                const uint32_t i = r * per_row + j;
-                const uint32_t p = (uint32_t) place[i];
-                if (p >= n_places) continue;
-                put_unit<T, LARGE>(out + (size_t) p * width + c, width - c, WEIGHTED ? scaled<T>(v, weights[i]) : v);
+        for (uint32_t r = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift); r < n_rows; r += row_blocks * (256u >> shift))
+            for (uint32_t c = sub * U; c < width; c += lanes * U) {
+                const auto v = unit_at<T, LARGE>(x + (size_t) r * width + c, width - c);
+                for (uint32_t j = 0; j < per_row; ++j) {
+                    const uint32_t i = r * per_row + j;
+                    const uint32_t p = (uint32_t) place[i];
+                    if (p >= n_places) continue;
+                    put_unit<T, LARGE>(out + (size_t) p * width + c, width - c, WEIGHTED ? scaled<T>(v, weights[i]) : v);
+                }
             }
-        }
     }
 
     // four entries' units under way
@@ -312,32 +312,31 @@ namespace splahip {
         constexpr uint32_t U        = kUnit<T>, AHEAD = 4;
         const uint32_t     lanes    = 1u << shift, sub = threadIdx.x & (lanes - 1u);
         const uint32_t     n_places = n_rows * per_row;
-        const uint32_t     r        = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift);
-        if (r >= n_rows) return;
-        for (uint32_t c = sub * U; c < width; c += lanes * U) {
-            float s[U] = {};
-            for (uint32_t j0 = 0; j0 < per_row; j0 += AHEAD) {
-                typename UnitOf<T>::mem v[AHEAD];
-                bool                    here[AHEAD];// (no entry: its weight does not count either)
+        for (uint32_t r = blockIdx.x * (256u >> shift) + (threadIdx.x >> shift); r < n_rows; r += gridDim.x * (256u >> shift))
+            for (uint32_t c = sub * U; c < width; c += lanes * U) {
+                float s[U] = {};
+                for (uint32_t j0 = 0; j0 < per_row; j0 += AHEAD) {
+                    typename UnitOf<T>::mem v[AHEAD];
+                    bool                    here[AHEAD];// (no entry: its weight does not count either)
 #pragma unroll
-                for (uint32_t j = 0; j < AHEAD; ++j) {
-                    const uint32_t p = j0 + j < per_row ? (uint32_t) place[r * per_row + j0 + j] : ~0u;
-                    here[j]          = p < n_places;
-                    if (here[j]) v[j] = unit_at<T, LARGE>(y + (size_t) p * width + c, width - c);
-                }
-#pragma unroll
-                for (uint32_t j = 0; j < AHEAD; ++j)
-                    if (here[j]) {
-                        const float w = WEIGHTED ? weights[r * per_row + j0 + j] : 1.0f;
-#pragma unroll
-                        for (uint32_t q = 0; q < U; ++q) s[q] = WEIGHTED ? fmaf(w, (float) v[j][q], s[q]) : s[q] + (float) v[j][q];
+                    for (uint32_t j = 0; j < AHEAD; ++j) {
+                        const uint32_t p = j0 + j < per_row ? (uint32_t) place[r * per_row + j0 + j] : ~0u;
+                        here[j]          = p < n_places;
+                        if (here[j]) v[j] = unit_at<T, LARGE>(y + (size_t) p * width + c, width - c);
                     }
-            }
-            typename UnitOf<T>::mem o;
 #pragma unroll
-            for (uint32_t q = 0; q < U; ++q) o[q] = (T) s[q];
-            put_unit<T, false>(out + (size_t) r * width + c, width - c, o);
-        }
+                    for (uint32_t j = 0; j < AHEAD; ++j)
+                        if (here[j]) {
+                            const float w = WEIGHTED ? weights[r * per_row + j0 + j] : 1.0f;
+#pragma unroll
+                            for (uint32_t q = 0; q < U; ++q) s[q] = WEIGHTED ? fmaf(w, (float) v[j][q], s[q]) : s[q] + (float) v[j][q];
+                        }
+                }
+                typename UnitOf<T>::mem o;
+#pragma unroll
+                for (uint32_t q = 0; q < U; ++q) o[q] = (T) s[q];
+                put_unit<T, false>(out + (size_t) r * width + c, width - c, o);
+            }
     }
 
     // One wavefront per row: an entry's weight gradient is reduced inside it.  UNITS units of dout's row stay in its registers (0: a row longer than eight per lane is read
@@ -354,48 +353,48 @@ namespace splahip {
             clear_rows(dy, min(offsets[n_experts], n_places), n_places, width, blockIdx.x - row_blocks, gridDim.x - row_blocks, 6);
             return;
         }
-        const uint32_t r = blockIdx.x * 4 + wave;
-        if (r >= n_rows) return;
-        const T*                grow = dout + (size_t) r * width;
-        typename UnitOf<T>::mem kept[KEPT];
-        if (UNITS)
+        for (uint32_t r = blockIdx.x * 4 + wave; r < n_rows; r += row_blocks * 4) {
+            const T*                grow = dout + (size_t) r * width;
+            typename UnitOf<T>::mem kept[KEPT];
+            if (UNITS)
 #pragma unroll
-            for (uint32_t u = 0; u < KEPT; ++u) {
-                const uint32_t c = (u * 64 + lane) * U;
-                if (c < width) kept[u] = unit_at<T, LARGE>(grow + c, width - c);
-            }
-        for (uint32_t j = 0; j < per_row; ++j) {
-            const uint32_t i   = r * per_row + j;
-            const uint32_t p   = (uint32_t) place[i];
-            float          dot = 0.0f;
-            if (p < n_places) {
-                const float w    = weights[i];
-                const T*    yrow = y + (size_t) p * width;
-                T*          drow = dy + (size_t) p * width;
-                auto        part = [&](uint32_t c, typename UnitOf<T>::mem g, typename UnitOf<T>::mem v) {
-#pragma unroll
-                    for (uint32_t q = 0; q < U; ++q) dot = fmaf((float) g[q], (float) v[q], dot);
-                    put_unit<T, LARGE>(drow + c, width - c, scaled<T>(g, w));
-                };
-                if (UNITS) {
-                    typename UnitOf<T>::mem v[KEPT];
-#pragma unroll
-                    for (uint32_t u = 0; u < KEPT; ++u) {
-                        const uint32_t c = (u * 64 + lane) * U;
-                        if (c < width) v[u] = unit_at<T, LARGE>(yrow + c, width - c);
-                    }
-#pragma unroll
-                    for (uint32_t u = 0; u < KEPT; ++u) {
-                        const uint32_t c = (u * 64 + lane) * U;
-                        if (c < width) part(c, kept[u], v[u]);
-                    }
-                } else {
-                    for (uint32_t c = lane * U; c < width; c += 64 * U) part(c, unit_at<T, false>(grow + c, width - c), unit_at<T, LARGE>(yrow + c, width - c));
+                for (uint32_t u = 0; u < KEPT; ++u) {
+                    const uint32_t c = (u * 64 + lane) * U;
+                    if (c < width) kept[u] = unit_at<T, LARGE>(grow + c, width - c);
                 }
+            for (uint32_t j = 0; j < per_row; ++j) {
+                const uint32_t i   = r * per_row + j;
+                const uint32_t p   = (uint32_t) place[i];
+                float          dot = 0.0f;
+                if (p < n_places) {
+                    const float w    = weights[i];
+                    const T*    yrow = y + (size_t) p * width;
+                    T*          drow = dy + (size_t) p * width;
+                    auto        part = [&](uint32_t c, typename UnitOf<T>::mem g, typename UnitOf<T>::mem v) {
 #pragma unroll
-                for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
+                        for (uint32_t q = 0; q < U; ++q) dot = fmaf((float) g[q], (float) v[q], dot);
+                        put_unit<T, LARGE>(drow + c, width - c, scaled<T>(g, w));
+                    };
+                    if (UNITS) {
+                        typename UnitOf<T>::mem v[KEPT];
+#pragma unroll
+                        for (uint32_t u = 0; u < KEPT; ++u) {
+                            const uint32_t c = (u * 64 + lane) * U;
+                            if (c < width) v[u] = unit_at<T, LARGE>(yrow + c, width - c);
+                        }
+#pragma unroll
+                        for (uint32_t u = 0; u < KEPT; ++u) {
+                            const uint32_t c = (u * 64 + lane) * U;
+                            if (c < width) part(c, kept[u], v[u]);
+                        }
+                    } else {
+                        for (uint32_t c = lane * U; c < width; c += 64 * U) part(c, unit_at<T, false>(grow + c, width - c), unit_at<T, LARGE>(yrow + c, width - c));
+                    }
+#pragma unroll
+                    for (int d = 32; d; d >>= 1) dot += __shfl_xor(dot, d);
+                }
+                if (lane == 0) dweights[i] = dot;
             }
-            if (lane == 0) dweights[i] = dot;
         }
     }
 
@@ -409,6 +408,7 @@ namespace splahip {
         SPLAHIP_REQUIRE(width < (1u << 30), "width: below 2^30");
         return SPLAHIP_OK;
     }
+    constexpr uint32_t kRowBlocks  = 1u << 20;// at most: a launch holds fewer than 2^32 threads
     constexpr uint32_t kTailBlocks = 128;// workgroups that clear the rows behind the last entry (none of them: they return at once)
     // A panel that the caches (256 MB behind the L2s) do not hold along with what else is read: streamed past the L2 (the gradient of 65536 x 2048 bf16 rows 125 -> 119 us).
     static bool large_panel(uint32_t n_places, uint32_t width, size_t element) { return (uint64_t) n_places * width * element > (128ull << 20); }
@@ -464,7 +464,7 @@ extern "C" int splahip_route_rows(int panel_type, uint32_t n_rows, uint32_t per_
     panel_dispatch(panel_type, [&](auto zero) {
         using T              = decltype(zero);
         const RowShape sh    = row_shape((width + kUnit<T> - 1) / kUnit<T>);
-        const uint32_t rows  = 256u >> sh.shift, blocks = (n_rows + rows - 1) / rows;
+        const uint32_t rows  = 256u >> sh.shift, blocks = std::min((n_rows + rows - 1) / rows, kRowBlocks);
         auto*          x     = static_cast<const T*>(d_x);
         auto*          out   = static_cast<T*>(d_out);
         const bool     large = large_panel(n_rows * per_row, width, sizeof(T));
@@ -487,7 +487,7 @@ extern "C" int splahip_route_back(int panel_type, uint32_t n_rows, uint32_t per_
     panel_dispatch(panel_type, [&](auto zero) {
         using T             = decltype(zero);
         const RowShape sh   = row_shape((width + kUnit<T> - 1) / kUnit<T>);
-        const uint32_t rows = 256u >> sh.shift, blocks = (n_rows + rows - 1) / rows;
+        const uint32_t rows = 256u >> sh.shift, blocks = std::min((n_rows + rows - 1) / rows, kRowBlocks);
         auto*          y    = static_cast<const T*>(d_y);
         auto*          out  = static_cast<T*>(d_out);
         const bool     large = large_panel(n_rows * per_row, width, sizeof(T));
@@ -507,7 +507,7 @@ extern "C" int splahip_route_back_grad(int panel_type, uint32_t n_rows, uint32_t
     SPLAHIP_REQUIRE(d_offsets && d_place && d_weights && d_dweights && (width == 0 || (d_y && d_dout && d_dy)), "null array");
     if (int st = ensure_device()) return st;
     hipStream_t    s      = as_stream(stream);
-    const uint32_t blocks = (n_rows + 3) / 4;
+    const uint32_t blocks = std::min((n_rows + 3) / 4, kRowBlocks);
     panel_dispatch(panel_type, [&](auto zero) {
         using T = decltype(zero);
         const uint32_t per_lane = (width + 64 * kUnit<T> - 1) / (64 * kUnit<T>);

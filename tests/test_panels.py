@@ -95,16 +95,17 @@ def test_c_entries_refuse():
 def test_clip_refuses_overlaps_and_limits():
     base = 1 << 40  # addresses that nothing reads: the checks come first
 
-    def clip(src, dst, n, types, limit=1.0):
+    def clip(src, dst, n, types, limit=1.0, norm=1 << 30, given=0):
         k = len(src)
         work = (C.c_uint64 * 4096)()
-        _fails("splahip_clip_global_norm", k, (C.c_void_p * k)(*src), (C.c_void_p * k)(*dst), (C.c_uint64 * k)(*n), (C.c_int * k)(*types), limit, 0,
-               C.cast(work, C.c_void_p), 4096 * 8, C.cast(work, C.c_void_p), None)
+        _fails("splahip_clip_global_norm", k, (C.c_void_p * k)(*src), (C.c_void_p * k)(*dst), (C.c_uint64 * k)(*n), (C.c_int * k)(*types), limit, given,
+               C.cast(work, C.c_void_p), 4096 * 8, C.c_void_p(norm), None)
 
     clip([base, base], [base, base], [4, 4], [0, 0])                         # the same array twice, in place
     clip([base, base + 64], [base, base + 12], [4, 4], [0, 0])               # results overlap by an element
     clip([base, base + 4096], [base + 4100, base + 8192], [4, 4], [0, 0])    # a result over another array
     clip([base], [base + 2], [4], [1])                                       # a result shifted into its own array
+    clip([base], [base], [4], [0], norm=base + 12, given=1)                  # the norm is one of the values it scales
     clip([base], [base], [4], [5])                                           # type
     clip([0], [base], [4], [0])                                              # null
     for limit in (-1.0, float("inf"), float("nan")):

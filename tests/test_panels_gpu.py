@@ -243,17 +243,35 @@ def test_product_needs():
 
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_product_keeps_bad_values_in_their_rows(dtype, bad):
+@pytest.mark.parametrize("rows,k,experts,n_in,n_out", [(70, 2, 3, 48, 40), (30, 2, 3, 72, 64), (70, 2, 3, 47, 41), (4000, 2, 3, 64, 2048), (4100, 1, 3, 250, 333)])
+def test_product_keeps_bad_values_in_their_rows(rows, k, experts, n_in, n_out, dtype, bad):
     """an infinity or NaN of one expert's row reaches that row's results (and that expert's dw), nothing beside it"""
-    plan, x, w, dy, offsets = _product_case(70, 2, 3, 48, 40, dtype, True)
-    y, dx, dw = _products(x, w, dy, offsets)
+    plan, x, w, dy, offsets = _product_case(rows, k, experts, n_in, n_out, dtype, False)
+    x, w, dy = x.cuda(), w.cuda(), dy.cuda()
+    y = kernels.expert_product(plan, x, w)
+    dx, dw = kernels.expert_product_grad(plan, x, w, dy)
     row = offsets[1]
     x[row, 7] = bad
-    got = kernels.expert_product(plan, x.cuda(), w.cuda()).cpu()
+    got = kernels.expert_product(plan, x, w)
     keep = torch.arange(x.shape[0]) != row
-    assert torch.equal(got[keep], y.to(dtype)[keep]) and not torch.isfinite(got[row]).all()
-    got_dx, got_dw = (t.cpu() for t in kernels.expert_product_grad(plan, x.cuda(), w.cuda(), dy.cuda()))
-    assert torch.equal(got_dx, dx.to(dtype)) and torch.equal(got_dw[[0, 2]], dw.to(dtype)[[0, 2]]) and torch.equal(got_dw[1, :, 8:], dw.to(dtype)[1, :, 8:])
+    assert torch.isfinite(y).all() and torch.equal(got[keep], y[keep]) and not torch.isfinite(got[row]).any()
+    got_dx, got_dw = kernels.expert_product_grad(plan, x, w, dy)
+    column = torch.arange(n_in) != 7
+    assert torch.equal(got_dx, dx) and torch.equal(got_dw[[0, 2]], dw[[0, 2]]) and torch.equal(got_dw[1][:, column], dw[1][:, column])
+    assert not torch.isfinite(got_dw[1, :, 7]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,experts,n_in,n_out", [(70, 2, 3, 48, 40), (30, 2, 3, 72, 64), (70, 2, 3, 47, 41), (4000, 2, 3, 64, 2048)])
+def test_product_of_subnormal_numbers(rows, k, experts, n_in, n_out, dtype):
+    """whole multiples of the type's smallest number times whole numbers: every sum is such a multiple, exactly"""
+    plan, x, w, dy, offsets = _product_case(rows, k, experts, n_in, n_out, dtype, True)
+    tiny = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}[dtype]
+    scaled = (x.double() * tiny).to(dtype)
+    assert torch.equal(torch.nan_to_num(scaled.double()), torch.nan_to_num(x.double()) * tiny)
+    y, dx, dw = _products(x, w, dy, offsets)
+    assert torch.equal(kernels.expert_product(plan, scaled.cuda(), w.cuda()).cpu(), (y * tiny).to(dtype))
+    assert torch.equal(kernels.expert_product_grad(plan, scaled.cuda(), w.cuda(), dy.cuda())[1].cpu(), (dw * tiny).to(dtype))
 
 
 def test_gradients_are_the_differences():
@@ -453,6 +471,32 @@ def test_same_results_every_time():
     t = _tensors([1_000_001, 77], [torch.float32, torch.float16])
     norms = {float(kernels.global_norm(t)) for _ in range(4)}
     assert len(norms) == 1
+
+
+def test_more_rows_than_a_launch_has_threads():
+    """70 M rows: a wavefront each would be more than 2^32 threads"""
+    rows = 70_000_000
+    e = torch.arange(rows, dtype=torch.int32, device="cuda")[:, None] % 2
+    plan = kernels.route_sort(e, 2)
+    assert plan.offsets.tolist() == [0, rows // 2, rows]
+    y = torch.ones(rows, 1, dtype=torch.bfloat16, device="cuda")
+    g = (torch.arange(rows, device="cuda") % 128).bfloat16()[:, None]
+    dy, dw = kernels.route_back_grad(plan, y, torch.ones(rows, 1, device="cuda"), g)
+    assert torch.equal(dw, g.float()) and torch.equal(dy[:rows // 2], g[0::2]) and torch.equal(dy[rows // 2:], g[1::2])
+    assert torch.equal(kernels.route_rows(plan, g), dy) and torch.equal(kernels.route_back(plan, dy), g)
+
+
+def test_panels_of_no_columns_and_no_rows():
+    plan = kernels.route_sort(torch.zeros(3, 2, dtype=torch.int32, device="cuda"), 2)
+    empty = torch.empty(3, 0, device="cuda")
+    assert kernels.route_rows(plan, empty).shape == (6, 0) and kernels.route_back(plan, torch.empty(6, 0, device="cuda")).shape == (3, 0)
+    dy, dw = kernels.route_back_grad(plan, torch.empty(6, 0, device="cuda"), torch.ones(3, 2, device="cuda"), empty)
+    assert dy.shape == (6, 0) and torch.equal(dw.cpu(), torch.zeros(3, 2))
+    plan = kernels.route_sort(torch.empty(0, 2, dtype=torch.int32, device="cuda"), 2)
+    x, w = torch.empty(0, 8, dtype=torch.bfloat16, device="cuda"), torch.ones(2, 16, 8, dtype=torch.bfloat16, device="cuda")
+    assert kernels.route_rows(plan, x).shape == (0, 8) and kernels.route_back(plan, x).shape == (0, 8) and kernels.expert_product(plan, x, w).shape == (0, 16)
+    dx, dw = kernels.expert_product_grad(plan, x, w, torch.empty(0, 16, dtype=torch.bfloat16, device="cuda"))
+    assert dx.shape == (0, 8) and not dw.any() and dw.shape == w.shape
 
 
 def test_panels_beyond_32_bit_offsets():
