@@ -59,7 +59,8 @@ def _sorted(e, n_experts):
 
 SORTS = [(0, 2, 4, 0, False), (1, 1, 1, 0, False), (1, 8, 8, 0, False), (5, 3, 7, 0.3, True), (64, 2, 8, 0, False), (63, 1, 2, 0, False), (2048, 1, 3, 0, False),
          (2049, 2, 65, 0.1, True), (5000, 8, 128, 0.1, False), (777, 5, 2048, 0, True), (300, 4, 16, 1.1, False), (1500, 7, 1, 0.5, False),
-         (0, 1, 1500, 0, False), (8192, 1, 512, 0.1, True), (8193, 1, 512, 0.1, True), (4096, 3, 700, 0.2, True), (30011, 2, 128, 0.05, True), (9000, 1, 1, 0.5, False)]
+         (0, 1, 1500, 0, False), (8192, 1, 512, 0.1, True), (8193, 1, 512, 0.1, True), (4096, 3, 700, 0.2, True), (30011, 2, 128, 0.05, True), (9000, 1, 1, 0.5, False), (100003, 1, 500, 0.1, True), (400009, 1, 512, 0.1, True),
+         (300007, 2, 5, 0.1, False)]
 
 
 @pytest.mark.parametrize("rows,k,experts,padding,strange", SORTS)
