@@ -8,9 +8,9 @@
 // Rows behind the last entry (offsets[n_experts] ..) become 0; an expert without rows has dw = 0.  fp32 sums in a fixed order, one rounding to the panel's
 // type.  fp32 panels are multiplied in full fp32 (v_mfma_f32_32x32x2_f32).
 #include "panel.hpp"
+
 #include <algorithm>
 #include <type_traits>
-
 
 namespace splahip {
 
@@ -285,6 +285,11 @@ namespace splahip {
     // instructions run from registers, the operands of the next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last
     // quarter: behind it every wavefront has read this step's two slabs, so the next two loads may overwrite them, and the next step's slabs have arrived (issued one
     // step ago, A's two steps ago).  The loads of the next tile's first slabs are under way while a tile's result is stored.
+    // Bound: in 16 bits the card's power.  32768 rows x 2048 x 4096 over 8 even experts, 256 x 256 tiles: 445 us = 1.23 PFLOP/s forward, 435 and 450 for the gradients, at 1.7 GHz
+    // (on zeros, which cost no power, 350 us = 1.57); 128 x 128 tiles 585 us: an operand's byte is used half as often.  fp32: the matrix cores, 8192 x 1024 x 1024 over 8
+    // experts 150 us = 115 TFLOP/s.  kElements at 16384 x 1001 x 1003: 370 and 240 TFLOP/s where 1000 x 1008 takes 640, misaligned 16-byte accesses being what costs.
+    // Small problems (4096 x 1024 x 1024 over 16 experts: 20 us) wait for the CUs that have two tiles.
+    //
     // 16 bytes of a result row, or as many of their elements as the row has left.  A large result passes the L2 by: it would push out the slabs that the workgroups share
     // (all of them store at about the same time).
     template<bool LARGE, typename T>
@@ -611,6 +616,8 @@ namespace splahip {
     // part of the matrix is read again, from the cache); its four wavefronts take the depth in turns of 128 bytes, so that a matrix row is read in runs of
     // 512, and go from memory to the matrix instruction without LDS: lane l holds row l % 16, 16 bytes of k from unit l / 16.  The wavefronts' sums are joined in LDS in
     // a fixed order.  Many small workgroups instead of a few that stay: what counts is bytes under way.
+    // 256 rows over 32 matrices of 2048 x 2048 bf16, none of it cached: 50 us = 5.4 TB/s (the tile kernel: 64); 2 rows through two of eight 2048 x 4096: 9 us (18).  One row block of
+    // 16 and 32 columns instead of 64: 61 us (the rows are read too often); through LDS in whole rows: 65.  From 24 rows per expert on the tile kernel is the faster one.
     __device__ __forceinline__ f32x4 matrix_step16(s16x8 a, s16x8 b, f32x4 c, bf16_t) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -738,7 +745,8 @@ namespace splahip {
     }
 
     static uint64_t matrix_tiles(const ProductArgs& g, uint64_t bm) { return g.n_experts * ((g.m + bm - 1) / bm) * ((g.n + bm - 1) / bm); }
-    // the size of tile that fills the card
+    // The size of tile that fills the card: 256 (128 in fp32) takes 0.76 of the time of the next smaller one if there are enough of them (200 here, 200 by the average of the rows in
+    // launch_of_type; 400 in fp32, two to a CU), up to twice the time if most CUs get none.
     static uint32_t matrix_grad_tile(const ProductArgs& g, uint32_t element, bool aligned) {
         if (element == 4) return matrix_tiles(g, 128) >= 400 ? 128 : 64;
         return aligned && matrix_tiles(g, 256) >= 200 ? 256 : 128;
