@@ -100,7 +100,8 @@ namespace splahip {
     template<typename P>
     __device__ __forceinline__ P* uniform(P* p) {// the same in every lane, as the compiler may not see
         const uint64_t v = (uint64_t) p;
-        return (P*) (((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32)) << 32) | (uint32_t) __builtin_amdgcn_readfirstlane((uint32_t) v));
+        const uint64_t u = ((uint64_t) (uint32_t) __builtin_amdgcn_readfirstlane((uint32_t) (v >> 32)) << 32) | (uint32_t) __builtin_amdgcn_readfirstlane((uint32_t) v);
+        return (P*) (__attribute__((address_space(1))) P*) u;// (global memory: not the flat accesses that a number turned pointer would get)
     }
 
     // Tile number t of a grid of row_tiles x col_tiles: H row tiles side by side, column by column, so that neighbouring tiles share both operands' slabs.
@@ -256,22 +257,28 @@ namespace splahip {
             for (uint32_t i = 0; i < kLoads; ++i)
                 load_to_lds<LOAD>(depth_of(i) < left ? reinterpret_cast<const char*>(base) + off[i] : reinterpret_cast<const char*>(zero_page), dst + i * (THREADS * kPiece));
         }
-        // kElements: into registers ..
-        static __device__ __forceinline__ void fetch(const T* base, const uint32_t (&off)[kLoads], uint32_t rows, uint32_t left, s16x8 (&r)[kLoads]) {
+        // kElements: into registers ..  A unit may reach beyond its row into the next one: elements behind `rows` belong to results that are not stored, elements of k behind `left` are
+        // cleared.  At the array's end it is read element by element.
+        static __device__ __forceinline__ void fetch(const T* base, const T* end, const uint32_t (&off)[kLoads], uint32_t left, s16x8 (&r)[kLoads]) {
+            constexpr uint32_t U = kUnit<T>;
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const T*       p   = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off[i]);
-                const uint32_t row = row_of(i) < rows ? row_of(i) : 0u, k = depth_of(i);
-                // elements of the unit that exist: a row of k ends at `left`, a row of rows at `rows`
-                const uint32_t have = DEPTH_CONTIGUOUS ? (k < left ? left - k : 0u) : (k < left ? rows - row : 0u);
-                if (have >= (uint32_t) kUnit<T>) r[i] = __builtin_bit_cast(s16x8, *reinterpret_cast<const typename UnitOf<T>::mem*>(p));
-                else {
-                    T v[kUnit<T>];
+                const T*       p = reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + off[i]);
+                const uint32_t k = depth_of(i);
+                r[i]             = s16x8{};
+                if (k >= left) continue;
+                if (p + U <= end) r[i] = __builtin_bit_cast(s16x8, *reinterpret_cast<const typename UnitOf<T>::mem*>(p));
+                else
 #pragma unroll
-                    for (uint32_t q = 0; q < (uint32_t) kUnit<T>; ++q) v[q] = q < have ? p[q] : (T) 0.0f;
-                    r[i] = *reinterpret_cast<const s16x8*>(v);
-                }
+                    for (uint32_t q = 0; q < U; ++q)
+                        if (p + q < end) r[i][q] = __builtin_bit_cast(short, p[q]);
             }
+            if (DEPTH_CONTIGUOUS && left < kStep<T>)
+#pragma unroll
+                for (uint32_t i = 0; i < kLoads; ++i)
+#pragma unroll
+                    for (uint32_t q = 0; q < U; ++q)
+                        if (depth_of(i) + q >= left) r[i][q] = 0;
         }
         // .. and on into LDS
         static __device__ __forceinline__ void put(const s16x8 (&r)[kLoads], T* slab) {
@@ -374,10 +381,12 @@ namespace splahip {
                     SlabB::load_last(B + s * move_b, off_b, depth - s * kStep<T>, dst_of(slot));
             }
         };
-        // kElements: a slab of each operand on its way
+        // kElements: a slab of each operand on its way, the operands' ends
+        const T* const end_a = static_cast<const T*>(g.a) + (size_t) g.n_places * (FORM == kMatrixGrad ? g.m : g.k);
+        const T* const end_b = static_cast<const T*>(g.b) + (FORM == kMatrixGrad ? (size_t) g.n_places * g.n : (size_t) g.n_experts * g.n * g.k);
         s16x8 ra[LOADS], rb[LOADS];
-        auto  fetch_a = [&](uint32_t s) { if (s < steps) SlabA::fetch(A + s * move_a, off_a, rows, min(kStep<T>, depth - s * kStep<T>), ra); };
-        auto  fetch_b = [&](uint32_t s) { if (s < steps) SlabB::fetch(B + s * move_b, off_b, cols, min(kStep<T>, depth - s * kStep<T>), rb); };
+        auto  fetch_a = [&](uint32_t s) { if constexpr (LOAD == kElements) if (s < steps) SlabA::fetch(A + s * move_a, end_a, off_a, min(kStep<T>, depth - s * kStep<T>), ra); };
+        auto  fetch_b = [&](uint32_t s) { if constexpr (LOAD == kElements) if (s < steps) SlabB::fetch(B + s * move_b, end_b, off_b, min(kStep<T>, depth - s * kStep<T>), rb); };
 
         if (!next()) return;
         slab_a(0, 0), slab_b(0, 1), slab_a(1, 2), slab_b(1, 3);
