@@ -622,11 +622,12 @@ namespace splahip {
 
     // ---- few rows per expert -----------------------------------------------------------------------------------------------------------------------------
     // Serving: every matrix is read for a few rows, the time is that of reading them.  A workgroup computes all rows of an expert x 16 NF columns, 32 at a time (for more, its
-    // part of the matrix is read again, from the cache); its four wavefronts take the depth in turns of 128 bytes, so that a matrix row is read in runs of
-    // 512, and go from memory to the matrix instruction without LDS: lane l holds row l % 16, 16 bytes of k from unit l / 16.  The wavefronts' sums are joined in LDS in
+    // part of the matrix is read again, from the cache); its WAVES wavefronts take the depth in turns of 128 bytes, so that a matrix row is read in runs of
+    // 512 and more, and go from memory to the matrix instruction without LDS: lane l holds row l % 16, 16 bytes of k from unit l / 16.  The wavefronts' sums are joined in LDS in
     // a fixed order.  Many small workgroups instead of a few that stay: what counts is bytes under way.
     // 256 rows over 32 matrices of 2048 x 2048 bf16, none of it cached: 50 us = 5.4 TB/s (the tile kernel: 64); 2 rows through two of eight 2048 x 4096: 9 us (18).  One row block of
-    // 16 and 32 columns instead of 64: 61 us (the rows are read too often); through LDS in whole rows: 65.  From 24 rows per expert on the tile kernel is the faster one.
+    // 16 and 32 columns instead of 64: 61 us (the rows are read too often); through LDS in whole rows: 65.  Where that leaves CUs without work, 16 columns and eight
+    // wavefronts (8 rows through 8 of 13 matrices of 4032 x 192: 14.0 -> 7.7 us).  From 24 rows per expert on the tile kernel is the faster one.
     __device__ __forceinline__ f32x4 matrix_step16(s16x8 a, s16x8 b, f32x4 c, bf16_t) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -642,16 +643,16 @@ namespace splahip {
 
     constexpr uint32_t kZeroBlocks = 64;// workgroups for the rows behind the last entry
 
-    template<typename T, uint32_t NF>
-    __global__ __launch_bounds__(256) void product_few_rows_kernel(const ProductArgs g, uint32_t col_tiles) {
+    template<typename T, uint32_t NF, uint32_t WAVES>
+    __global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const ProductArgs g, uint32_t col_tiles) {
         constexpr uint32_t MF = 2, U = kUnit<T>, CHUNK = 8 * U, AHEAD = 2;// chunks of a wavefront under way
-        __shared__ f32x4   part[4][NF * MF][64];
+        __shared__ f32x4   part[WAVES][NF * MF][64];
         const uint32_t     lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
         const uint32_t     expert = blockIdx.x / col_tiles;
         typedef T          four __attribute__((ext_vector_type(4)));
         if (expert >= g.n_experts) {
-            const uint64_t end = (uint64_t) g.n_places * (g.n / 4), step = (uint64_t) (gridDim.x - g.n_experts * col_tiles) * 256;
-            for (uint64_t i = (uint64_t) bounded(g.offsets, g.n_experts, g.n_experts, g.n_places) * (g.n / 4) + (blockIdx.x - g.n_experts * col_tiles) * 256 + threadIdx.x; i < end; i += step)
+            const uint64_t end = (uint64_t) g.n_places * (g.n / 4), step = (uint64_t) (gridDim.x - g.n_experts * col_tiles) * (WAVES * 64);
+            for (uint64_t i = (uint64_t) bounded(g.offsets, g.n_experts, g.n_experts, g.n_places) * (g.n / 4) + (blockIdx.x - g.n_experts * col_tiles) * (WAVES * 64) + threadIdx.x; i < end; i += step)
                 reinterpret_cast<four*>(g.c)[i] = four{};
             return;
         }
@@ -667,7 +668,7 @@ namespace splahip {
 #pragma unroll
             for (uint32_t i = 0; i < MF; ++i) x[i] = static_cast<const T*>(g.a) + (size_t) (row0 + min(i * 16 + (lane & 15u), rows - 1)) * g.k + (lane >> 4) * U;
             f32x4 acc[MF][NF] = {};
-            for (uint32_t k0 = wave * CHUNK; k0 < depth; k0 += 4 * CHUNK * AHEAD) {
+            for (uint32_t k0 = wave * CHUNK; k0 < depth; k0 += WAVES * CHUNK * AHEAD) {
                 s16x8 a[AHEAD][2][NF], b[AHEAD][2][MF];
 #pragma unroll
                 for (uint32_t c = 0; c < AHEAD; ++c) {
@@ -675,14 +676,14 @@ namespace splahip {
                     for (uint32_t j = 0; j < NF; ++j)
 #pragma unroll
                         for (uint32_t h = 0; h < 2; ++h) {
-                            const uint32_t k = k0 + c * 4 * CHUNK + h * 4 * U;
+                            const uint32_t k = k0 + c * WAVES * CHUNK + h * 4 * U;
                             a[c][h][j]       = k + (lane >> 4) * U < depth ? *reinterpret_cast<const s16x8*>(w[j] + k) : s16x8{};// (the depth comes in whole units)
                         }
 #pragma unroll
                     for (uint32_t i = 0; i < MF; ++i)
 #pragma unroll
                         for (uint32_t h = 0; h < 2; ++h) {
-                            const uint32_t k = k0 + c * 4 * CHUNK + h * 4 * U;
+                            const uint32_t k = k0 + c * WAVES * CHUNK + h * 4 * U;
                             b[c][h][i]       = k + (lane >> 4) * U < depth ? *reinterpret_cast<const s16x8*>(x[i] + k) : s16x8{};
                         }
                 }
@@ -701,8 +702,10 @@ namespace splahip {
 #pragma unroll
                 for (uint32_t j = 0; j < NF; ++j) part[wave][i * NF + j][lane] = acc[i][j];
             __syncthreads();
-            for (uint32_t f = wave; f < MF * NF; f += 4) {
-                const f32x4    sum = (part[0][f][lane] + part[1][f][lane]) + (part[2][f][lane] + part[3][f][lane]);
+            for (uint32_t f = wave; f < MF * NF; f += WAVES) {
+                f32x4 sum = part[0][f][lane];
+#pragma unroll
+                for (uint32_t w = 1; w < WAVES; ++w) sum += part[w][f][lane];
                 const uint32_t m = f / NF * 16 + (lane & 15u), n = n0 + f % NF * 16 + (lane >> 4) * 4;
                 if (m < rows && n < g.n) {// (columns come in fours)
                     four c;
@@ -714,11 +717,11 @@ namespace splahip {
         }
     }
 
-    template<typename T, uint32_t NF>
+    template<typename T, uint32_t NF, uint32_t WAVES>
     static int launch_few_rows(const ProductArgs& g, hipStream_t s) {
         const uint64_t col_tiles = (g.n + 16 * NF - 1) / (16 * NF), blocks = g.n_experts * col_tiles + kZeroBlocks;
         SPLAHIP_REQUIRE(blocks < (1ull << 31), "too many tiles for one launch");
-        product_few_rows_kernel<T, NF><<<(uint32_t) blocks, 256, 0, s>>>(g, (uint32_t) col_tiles);
+        product_few_rows_kernel<T, NF, WAVES><<<(uint32_t) blocks, WAVES * 64, 0, s>>>(g, (uint32_t) col_tiles);
         SPLAHIP_TRY(hipGetLastError());
         return SPLAHIP_OK;
     }
@@ -798,7 +801,11 @@ namespace splahip {
             auto tiles = [&](uint64_t bm) { return (g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
             if constexpr (FORM == kForward)
                 if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts && g.n_experts * (uint64_t) (g.n / 32 + 1) < (1u << 23))// (a launch holds fewer than 2^32 threads)
-                    return std::min(g.n_places, g.n_experts) * (uint64_t) (g.n / 64) >= 1024 ? launch_few_rows<T, 4>(g, s) : launch_few_rows<T, 2>(g, s);
+{
+                    const uint64_t rows = std::min(g.n_places, g.n_experts);// experts that have some, at most
+                    if (rows * (g.n / 64) >= 1024) return launch_few_rows<T, 4, 4>(g, s);
+                    return rows * (g.n / 32) >= 192 ? launch_few_rows<T, 2, 4>(g, s) : launch_few_rows<T, 1, 8>(g, s);
+                }
             if constexpr (sizeof(T) == 4) {
                 const bool large = tiles(128) >= 400;
                 if (aligned) return large ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s);

@@ -158,7 +158,8 @@ def test_back_without_any_entry_is_zero():
 # than a wavefront has lanes
 PRODUCTS = [(1, 1, 1, 1, 1), (1, 2, 8, 64, 96), (1, 8, 8, 512, 256), (4, 2, 3, 33, 17), (16, 1, 1, 64, 64), (17, 1, 1, 128, 128), (64, 4, 32, 256, 192), (100, 3, 130, 40, 56),
             (255, 1, 1, 96, 64), (256, 1, 1, 256, 256), (257, 1, 1, 264, 520), (513, 2, 2, 128, 320), (333, 3, 5, 250, 333), (700, 2, 3, 512, 512), (1500, 2, 4, 1000, 264),
-            (31, 2, 4, 2056, 72), (2000, 1, 300, 72, 136), (5000, 2, 2, 40, 56), (5000, 2, 3, 33, 65), (3001, 1, 1, 136, 72)]
+            (31, 2, 4, 2056, 72), (2000, 1, 300, 72, 136), (5000, 2, 2, 40, 56), (5000, 2, 3, 33, 65), (3001, 1, 1, 136, 72), (64, 4, 64, 128, 1024), (50, 8, 20, 2072, 24),
+            (9, 2, 6, 1096, 1040)]
 
 
 def _product_case(rows, k, experts, n_in, n_out, dtype, whole, seed=9):
