@@ -786,10 +786,8 @@ namespace splahip {
         if constexpr (FORM == kMatrixGrad) {
             const uint32_t bm = matrix_grad_tile(g, sizeof(T), aligned);
             if constexpr (sizeof(T) == 4) {
-                if (g.splits > 1) {
-                    if (bm == 128) return aligned ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, false, true>(g, s) : launch_tiles<T, FORM, kWords, 128, 2, 2, 2, false, true>(g, s);
+                if (g.splits > 1)// (more than 256 tiles of 128 are not split)
                     return aligned ? launch_tiles<T, FORM, kUnits, 64, 2, 2, 4, false, true>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4, false, true>(g, s);
-                }
                 if (bm == 128) return aligned ? launch_tiles<T, FORM, kUnits, 128, 2, 2, 2, true>(g, s) : launch_tiles<T, FORM, kWords, 128, 2, 2, 2, true>(g, s);
                 return aligned ? launch_tiles<T, FORM, kUnits, 64, 2, 2, 4>(g, s) : launch_tiles<T, FORM, kWords, 64, 2, 2, 4>(g, s);
             } else {

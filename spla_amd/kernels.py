@@ -257,7 +257,8 @@ _PANEL_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 _entries = {}
-_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle without a Python stream object around it (a fifth of a small call's time)
+# the current stream's handle and device without the Python objects and checks around them (a fifth of a small call's time; the tensors have initialised the GPU)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _launch(device, name, *args):
@@ -266,7 +267,7 @@ def _launch(device, name, *args):
     if fn is None:
         fn = _entries[name] = getattr(_lib.load(), name)
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
@@ -383,16 +384,18 @@ def route_back_grad(plan: RoutePlan, y: torch.Tensor, weights: torch.Tensor, dou
 
 
 def _matrices(plan, w, dtype):
-    if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.shape[0] != plan.n_experts or w.shape[1] < 1 or w.shape[2] < 1:
-        raise ValueError(f"w: matrices [{plan.n_experts}, n_out, n_in] expected, not {tuple(w.shape) if isinstance(w, torch.Tensor) else type(w).__name__}")
-    return _checked("w", w, dtype, w.shape, plan.device)
+    """the address of w [n_experts, n_out, n_in], n_out and n_in"""
+    shape = w.shape if isinstance(w, torch.Tensor) else ()
+    if len(shape) != 3 or shape[0] != plan.n_experts or shape[1] < 1 or shape[2] < 1:
+        raise ValueError(f"w: matrices [{plan.n_experts}, n_out, n_in] expected, not {tuple(shape) if isinstance(w, torch.Tensor) else type(w).__name__}")
+    return _checked("w", w, dtype, shape, plan.device), shape[1], shape[2]
 
 
 def expert_product(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """y[p] = w[e] @ x[p] for the places p of expert e: x [n_places, n_in] in expert order, w [n_experts, n_out, n_in] of the same type.  Rows behind the last
     entry are not read and become 0."""
-    t, src_w = _panel_type("x", x), _matrices(plan, w, x.dtype)
-    n_out, n_in = w.shape[1:]
+    t = _panel_type("x", x)
+    src_w, n_out, n_in = _matrices(plan, w, x.dtype)
     src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
     y = torch.empty(plan.n_places, n_out, dtype=x.dtype, device=plan.device)
     _launch(plan.device, "splahip_expert_product", t, plan.n_places, plan.n_experts, n_in, n_out, plan.offsets.data_ptr(), src, src_w, y.data_ptr())
@@ -402,8 +405,8 @@ def expert_product(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor) -> torch.T
 def expert_product_grad(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor, dy: torch.Tensor, need=(True, True)):
     """The gradients (dx, dw) of expert_product(plan, x, w): dx[p] = w[e]^T @ dy[p] (0 behind the last entry), dw[e] = sum of dy[p] x[p]^T over the expert's
     places (0 for an expert without any).  need: which of the two to compute, None stands in the place of the other."""
-    t, src_w = _panel_type("x", x), _matrices(plan, w, x.dtype)
-    n_out, n_in = w.shape[1:]
+    t = _panel_type("x", x)
+    src_w, n_out, n_in = _matrices(plan, w, x.dtype)
     src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
     src_dy = _checked("dy", dy, x.dtype, (plan.n_places, n_out), plan.device)
     dx = dw = None
