@@ -76,25 +76,44 @@ namespace splahip {
         return before + inc - x;
     }
 
-    // 64 experts a workgroup, one per lane; the wavefronts share the tiles in contiguous parts: the counts become exclusive prefixes over the tiles, their sums the totals
+    // 16 experts a workgroup, the tiles in 64 contiguous parts: the counts become exclusive prefixes over the tiles, their sums the totals.  (64 experts and 16 parts: 4.7 instead of
+    // 3.5 us at 256 tiles x 128 experts, the loads of a part coming one after another.)
     __global__ __launch_bounds__(1024) void route_scan_kernel(uint32_t n_tiles, uint32_t n_experts, uint32_t* __restrict__ counts, uint32_t* __restrict__ totals) {
-        __shared__ uint32_t part[16][64];
-        const uint32_t      lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
-        const uint32_t      per = (n_tiles + 15) / 16, t0 = min(wave * per, n_tiles), t1 = min(t0 + per, n_tiles);
-        uint32_t            sum = 0;
-        if (e < n_experts)
-#pragma unroll 8
-            for (uint32_t t = t0; t < t1; ++t) sum += counts[(size_t) t * n_experts + e];
-        part[wave][lane] = sum;
-        __syncthreads();
-        uint32_t at = 0, all = 0;
+        __shared__ uint32_t part[16][65];
+        const uint32_t      lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, col = threadIdx.x & 15u, g = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
+        const uint32_t      per = (n_tiles + 63) / 64, t0 = min(g * per, n_tiles), t1 = min(t0 + per, n_tiles);
+        uint32_t            sum = 0, kept[8];// a part of up to 8 tiles stays in registers
+        const bool          few = per <= 8;
+        if (e < n_experts) {
+            if (few)
 #pragma unroll
-        for (uint32_t w = 0; w < 16; ++w) {
-            at += w < wave ? part[w][lane] : 0u;
-            all += part[w][lane];
+                for (uint32_t i = 0; i < 8; ++i) kept[i] = t0 + i < t1 ? counts[(size_t) (t0 + i) * n_experts + e] : 0u, sum += kept[i];
+            else
+#pragma unroll 8
+                for (uint32_t t = t0; t < t1; ++t) sum += counts[(size_t) t * n_experts + e];
         }
+        part[col][g] = sum;
+        __syncthreads();
+        const uint32_t own = part[wave][lane];// a wavefront scans an expert's parts
+        uint32_t       inc = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t up = __shfl_up(inc, d);
+            if (lane >= (uint32_t) d) inc += up;
+        }
+        part[wave][lane] = inc - own;
+        if (lane == 63 && blockIdx.x * 16 + wave < n_experts) totals[blockIdx.x * 16 + wave] = inc;
+        __syncthreads();
         if (e >= n_experts) return;
-        if (wave == 0) totals[e] = all;
+        uint32_t at = part[col][g];
+        if (few) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                if (t0 + i < t1) counts[(size_t) (t0 + i) * n_experts + e] = at;
+                at += kept[i];
+            }
+            return;
+        }
 #pragma unroll 8
         for (uint32_t t = t0; t < t1; ++t) {
             const uint32_t c                       = counts[(size_t) t * n_experts + e];
@@ -447,7 +466,7 @@ extern "C" int splahip_route_sort(uint32_t n_rows, uint32_t per_row, uint32_t n_
     uint32_t* counts = static_cast<uint32_t*>(d_workspace);
     uint32_t* totals = counts + (size_t) n_experts * tiles;
     if (tiles) route_count_kernel<<<tiles, kSortThreads, 0, s>>>(n, n_experts, d_experts, counts);
-    route_scan_kernel<<<(n_experts + 63) / 64, 1024, 0, s>>>(tiles, n_experts, counts, totals);
+    route_scan_kernel<<<(n_experts + 15) / 16, 1024, 0, s>>>(tiles, n_experts, counts, totals);
     auto* place_kernel = n_experts <= 512 ? route_place_kernel<512> : route_place_kernel<kMaxExperts>;
     place_kernel<<<tiles ? tiles : 1, kSortThreads, 0, s>>>(n, n_experts, bits, d_experts, counts, totals, d_offsets, d_order, d_place);
     SPLAHIP_TRY(hipGetLastError());

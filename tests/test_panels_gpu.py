@@ -463,6 +463,23 @@ def test_on_another_stream_and_in_a_graph():
                 assert torch.equal(a, b)
 
 
+def test_calls_on_two_streams_at_once():
+    """two steps on different inputs under way together, each as it is alone"""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    inputs = [_layer_inputs(torch.bfloat16, True, rows=2000 + 700 * i, k=2, experts=6 + i, n=128, hidden=256) for i in range(2)]
+    alone = [_layer(*args, experts, 1.0) for args, experts in inputs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        together = []
+        for side, (args, experts) in zip(sides, inputs):
+            with torch.cuda.stream(side):
+                together.append([_layer(*args, experts, 1.0) for _ in range(2)])
+        torch.cuda.synchronize()
+        for want, runs in zip(alone, together):
+            for got in runs:
+                assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(want, got))
+
+
 def test_same_results_every_time():
     plan, x, w, dy, _ = _product_case(900, 2, 4, 512, 256, torch.bfloat16, False)
     x, w, dy = x.cuda(), w.cuda(), dy.cuda()
