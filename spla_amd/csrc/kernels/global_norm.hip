@@ -16,19 +16,21 @@
 
 namespace splahip {
 
-    constexpr uint32_t kBatch = 128;// arrays per launch: 3.7 KB of arguments
+    constexpr uint32_t kBatch = 128, kSmallBatch = 16;// arrays per launch: 3.7 KB of arguments, or 0.5 where they do (each launch copies them)
 
+    template<uint32_t N>
     struct NormBatch {
-        const void* src[kBatch];
-        void*       dst[kBatch];
-        uint64_t    n[kBatch];
-        uint32_t    first[kBatch + 1];// first chunk of array i, ascending; [count] = chunks of the launch
-        uint8_t     type[kBatch];
+        const void* src[N];
+        void*       dst[N];
+        uint64_t    n[N];
+        uint32_t    first[N + 1];// first chunk of array i, ascending; [count] = chunks of the launch
+        uint8_t     type[N];
         uint32_t    count;
     };
 
     // which array chunk b belongs to
-    __device__ __forceinline__ uint32_t array_of(const NormBatch& a, uint32_t b) {
+    template<uint32_t N>
+    __device__ __forceinline__ uint32_t array_of(const NormBatch<N>& a, uint32_t b) {
         uint32_t lo = 0, hi = a.count;
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) >> 1;
@@ -80,7 +82,8 @@ namespace splahip {
         return s0 + s1;
     }
 
-    __global__ __launch_bounds__(256) void norm_partials_kernel(const NormBatch a, uint32_t chunk, double* __restrict__ partials) {
+    template<uint32_t N>
+    __global__ __launch_bounds__(256) void norm_partials_kernel(const NormBatch<N> a, uint32_t chunk, double* __restrict__ partials) {
         const uint32_t i   = array_of(a, blockIdx.x);
         const uint64_t at  = (uint64_t) (blockIdx.x - a.first[i]) * chunk;
         const uint64_t len = min(a.n[i] - at, (uint64_t) chunk);
@@ -136,8 +139,8 @@ namespace splahip {
             store_unit<T>(y + c, left, v);
         }
     }
-    template<Scaling HOW>
-    __device__ __forceinline__ void chunk_scale_any(const NormBatch& a, uint32_t i, uint64_t at, uint64_t len, double factor) {
+    template<Scaling HOW, uint32_t N>
+    __device__ __forceinline__ void chunk_scale_any(const NormBatch<N>& a, uint32_t i, uint64_t at, uint64_t len, double factor) {
         if (a.type[i] == SPLAHIP_PANEL_FLOAT) chunk_scale<float, HOW>(static_cast<const float*>(a.src[i]) + at, static_cast<float*>(a.dst[i]) + at, len, factor);
         else if (a.type[i] == SPLAHIP_PANEL_HALF)
             chunk_scale<fp16_t, HOW>(static_cast<const fp16_t*>(a.src[i]) + at, static_cast<fp16_t*>(a.dst[i]) + at, len, factor);
@@ -146,7 +149,8 @@ namespace splahip {
     }
 
     // the factor is rounded to 32 bits once, each product to 32 bits and to the array's type
-    __global__ __launch_bounds__(256) void norm_scale_kernel(const NormBatch a, uint32_t chunk, float limit, const float* __restrict__ norm32,
+    template<uint32_t N>
+    __global__ __launch_bounds__(256) void norm_scale_kernel(const NormBatch<N> a, uint32_t chunk, float limit, const float* __restrict__ norm32,
                                                              const double* __restrict__ norm64) {
         const double   norm   = norm64 ? *norm64 : (double) *norm32;
         const bool     same   = !(norm > (double) limit) || norm == INFINITY;// (a NaN compares false)
@@ -176,9 +180,9 @@ namespace splahip {
     }
 
     // launches f(batch, chunks, chunks before it) for the arrays in batches
-    template<typename F>
-    static void for_batches(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types, uint32_t chunk, F&& f) {
-        NormBatch a;
+    template<uint32_t N, typename F>
+    static void for_batches_of(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types, uint32_t chunk, F&& f) {
+        NormBatch<N> a;
         a.count        = 0;
         uint64_t done  = 0;
         uint32_t first = 0;
@@ -192,7 +196,7 @@ namespace splahip {
                 first += (uint32_t) ((lengths[i] + chunk - 1) / chunk);
                 ++a.count;
             }
-            if (a.count && (a.count == kBatch || i + 1 == n_arrays)) {
+            if (a.count && (a.count == N || i + 1 == n_arrays)) {
                 a.first[a.count] = first;
                 f(a, first, done);
                 done += first;
@@ -200,6 +204,13 @@ namespace splahip {
                 first   = 0;
             }
         }
+    }
+
+    template<typename F>
+    static void for_batches(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types, uint32_t chunk, F&& f) {
+        if (n_arrays <= kSmallBatch) for_batches_of<kSmallBatch>(n_arrays, src, dst, lengths, types, chunk, f);
+        else
+            for_batches_of<kBatch>(n_arrays, src, dst, lengths, types, chunk, f);
     }
 
     static int check_arrays(uint32_t n_arrays, const void* const* ptrs, const uint64_t* lengths, const int* types) {
@@ -264,7 +275,7 @@ extern "C" int splahip_global_norm(uint32_t n_arrays, const void* const* h_array
     double*        partials = norm64 + 1;
     const uint32_t chunk    = chunk_elements(total_elements(n_arrays, h_lengths));
     uint64_t       n        = 0;
-    for_batches(n_arrays, h_arrays, nullptr, h_lengths, h_types, chunk, [&](const NormBatch& a, uint32_t chunks, uint64_t before) {
+    for_batches(n_arrays, h_arrays, nullptr, h_lengths, h_types, chunk, [&](const auto& a, uint32_t chunks, uint64_t before) {
         norm_partials_kernel<<<chunks, 256, 0, s>>>(a, chunk, partials + before);
         n = before + chunks;
     });
@@ -288,7 +299,7 @@ extern "C" int splahip_clip_global_norm(uint32_t n_arrays, const void* const* h_
     if (int st = ensure_device()) return st;
     hipStream_t    s     = as_stream(stream);
     const uint32_t chunk = chunk_elements(total_elements(n_arrays, h_lengths));
-    for_batches(n_arrays, h_arrays, h_out, h_lengths, h_types, chunk, [&](const NormBatch& a, uint32_t chunks, uint64_t) {
+    for_batches(n_arrays, h_arrays, h_out, h_lengths, h_types, chunk, [&](const auto& a, uint32_t chunks, uint64_t) {
         norm_scale_kernel<<<chunks, 256, 0, s>>>(a, chunk, limit, d_norm, norm_given ? nullptr : static_cast<const double*>(d_workspace));
     });
     SPLAHIP_TRY(hipGetLastError());

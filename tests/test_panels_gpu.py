@@ -306,7 +306,7 @@ def _norm(tensors):
 
 
 LISTS = [([1], [torch.float32]), ([(3, 5), 0, 7], [torch.bfloat16, torch.float32, torch.float16]), ([2047, 2049, 1], DTYPES), ([70001] * 5, [torch.bfloat16] * 5),
-         ([(i % 13) * 3 for i in range(300)], [DTYPES[i % 3] for i in range(300)]), ([5_000_003, 4096], [torch.float32, torch.bfloat16]), ([0, 0], [torch.float32] * 2)]
+         ([(i % 13) * 3 for i in range(300)], [DTYPES[i % 3] for i in range(300)]), ([5_000_003, 4096], [torch.float32, torch.bfloat16]), ([513] * 16, [DTYPES[i % 3] for i in range(16)]), ([513] * 17, [DTYPES[i % 3] for i in range(17)]), ([0, 0], [torch.float32] * 2)]
 
 
 @pytest.mark.parametrize("sizes,dtypes", LISTS)
