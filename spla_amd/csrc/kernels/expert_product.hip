@@ -288,15 +288,6 @@ namespace splahip {
     };
 
     // ---- the kernel --------------------------------------------------------------------------------------------------------------------------------------
-    // A workgroup stays and computes one BM x BM tile after another, WM x WN wavefronts side by side.  A step of k is four quarters of two units: while a quarter's matrix
-    // instructions run from registers, the operands of the next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last
-    // quarter: behind it every wavefront has read this step's two slabs, so the next two loads may overwrite them, and the next step's slabs have arrived (issued one
-    // step ago, A's two steps ago).  The loads of the next tile's first slabs are under way while a tile's result is stored.
-    // Bound: in 16 bits the card's power.  32768 rows x 2048 x 4096 over 8 even experts, 256 x 256 tiles: 445 us = 1.23 PFLOP/s forward, 435 and 450 for the gradients, at 1.7 GHz
-    // (on zeros, which cost no power, 350 us = 1.57); 128 x 128 tiles 585 us: an operand's byte is used half as often.  fp32: the matrix cores, 8192 x 1024 x 1024 over 8
-    // experts 150 us = 115 TFLOP/s.  kElements at 16384 x 1001 x 1003: 370 and 240 TFLOP/s where 1000 x 1008 takes 640, misaligned 16-byte accesses being what costs.
-    // Small problems (4096 x 1024 x 1024 over 16 experts: 20 us) wait for the CUs that have two tiles.
-    //
     // 16 bytes of a result row, or as many of their elements as the row has left.  A large result passes the L2 by: it would push out the slabs that the workgroups share
     // (all of them store at about the same time).
     template<bool LARGE, typename T>
@@ -307,8 +298,7 @@ namespace splahip {
             else
                 *to = __builtin_bit_cast(typename UnitOf<T>::mem, c);
         } else {
-            T v[kUnit<T>];
-            *reinterpret_cast<s16x8*>(v) = c;
+            const auto v = __builtin_bit_cast(typename UnitOf<T>::mem, c);
 #pragma unroll
             for (uint32_t q = 0; q < (uint32_t) kUnit<T>; ++q)
                 if (q < left) p[q] = v[q];
@@ -322,6 +312,16 @@ namespace splahip {
         uint32_t rows, cols, depth;
     };
 
+    // A workgroup stays and computes one BM x BM tile after another, WM x WN wavefronts side by side.  A step of k is four quarters of two units: while a quarter's matrix
+    // instructions run from registers, the operands of the next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last
+    // quarter: behind it every wavefront has read this step's two slabs, so the next two loads may overwrite them, and the next step's slabs have arrived (issued one
+    // step ago, A's two steps ago).  The loads of the next tile's first slabs are under way while a tile's result is stored.
+    // Bound: in 16 bits the card's power.  32768 rows x 2048 x 4096 over 8 even experts, 256 x 256 tiles: 445 us = 1.23 PFLOP/s forward, 435 and 450 for the gradients, at 1.7 GHz
+    // (on zeros, which cost no power, 350 us = 1.57); 128 x 128 tiles 585 us: an operand's byte is used half as often.  fp32: the matrix cores, 8192 x 1024 x 1024 over 8
+    // experts 150 us = 115 TFLOP/s.  kElements at 16384 x 1001 x 1003: 400, 400 and 515 TFLOP/s (forward, dx, dw) where 1000 x 1008
+    // has 650, 650 and 755: its slabs go through registers, with misaligned 16-byte accesses; which of the two costs was not measured apart.
+    // Small problems (4096 x 1024 x 1024 over 16 experts: 20 us) wait for the CUs that have two tiles.
+    //
     // take(tile): the workgroup's next tile, false behind the last.  O: the result's type, T or (partial sums) float
     template<typename T, typename O, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, typename TAKE>
     __device__ __forceinline__ void run_tiles(const ProductArgs& g, T* lds, TAKE&& take) {
@@ -528,7 +528,8 @@ namespace splahip {
     }
 
     // SPLIT: the tiles left over when every workgroup has had the same number are cut in four, if there are few of them: most CUs would wait for a whole tile's time
-    // otherwise (132 row tiles x 16 columns on 256 CUs: nine tiles' time for 8.25 tiles' work).
+    // otherwise (132 row tiles x 16 columns on 256 CUs: nine tiles' time for 8.25 tiles' work; both gradients of 32768 x 2048 x 1024 over 32
+    // experts 307 -> 301 us, 8192 x 1024 x 1024 over 8 in fp32 192 -> 152).
     template<typename T, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, uint32_t OCC, bool SPLIT, bool PARTIAL>
     __global__ __launch_bounds__(WM* WN * 64, OCC) void product_kernel(const ProductArgs g, uint32_t col_tiles) {
         __shared__ __align__(1024) T lds[5 * BM * kStep<T>];
