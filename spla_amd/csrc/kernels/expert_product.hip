@@ -198,7 +198,8 @@ namespace splahip {
 
     // ---- from memory to LDS ------------------------------------------------------------------------------------------------------------------------------
     // kUnits: 16 bytes per lane straight into LDS; operands, rows and the result begin at multiples of 16 bytes.
-    // kWords: 4 bytes per lane straight into LDS; fp32 of any sizes.
+    // kWords: 4 bytes per lane straight into LDS; fp32 of any sizes (8000 rows x 1001 x 1003 over 8, forward, dx, dw: 168, 162, 144 us; as kElements 267, 226, 160; 4800 rows x
+    // 250 x 333 over 5: 16, 20, 21 us against 21, 24, 22, and 14, 17, 19 as kUnits at 252 x 336).
     // kElements: through registers, 16 bytes per lane from any address, the ends of rows element by element; 16-bit elements of odd sizes or alignment.
     enum Load { kUnits, kWords, kElements };
 
