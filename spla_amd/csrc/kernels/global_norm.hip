@@ -1,7 +1,10 @@
 // global_norm.hip — the 2-norm over many arrays as if they were one, and the arrays scaled down to a largest norm: the reduction of splahip_reduce over a list
 // of panels of mixed element types, whose result stays on the device.
 //
-//   norm = sqrt(sum over all arrays of x^2),  out = x * min(1, limit / norm)  (a norm that is not finite scales nothing)
+//   norm = sqrt(sum over all arrays of x^2),  out = x * min(1, limit / norm)
+//
+// The norm is used in 64 bits, where only a NaN or infinity among the values makes it one: that scales nothing.  Rounded to 32 bits it is infinity beyond FLT_MAX, while
+// the values are scaled all the same.  A norm that the caller gives has 32 bits: NaN and infinity scale nothing.
 //
 // Squares are taken and summed in 64 bits: the square of an fp32 value is exact there and no sum of them leaves the range, so neither a large gradient
 // overflows nor do many small ones get lost.  Every partial sum has its own word and a fixed order: the norm is the same from run to run.

@@ -449,7 +449,7 @@ def _arrays(name, tensors):
 
 def global_norm(tensors) -> torch.Tensor:
     """The 2-norm over all elements of all tensors (a list of contiguous float32 / float16 / bfloat16 tensors of any shapes on one device), a float32 scalar on
-    that device.  Squares and sums in 64 bits; the order of the sum is fixed."""
+    that device (infinity for a norm beyond float32).  Squares and sums in 64 bits; the order of the sum is fixed."""
     tensors = list(tensors)
     if not tensors:
         raise ValueError("tensors: at least one expected")
@@ -462,8 +462,9 @@ def global_norm(tensors) -> torch.Tensor:
 
 
 def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None) -> torch.Tensor:
-    """Scale the tensors by min(1, limit / norm), in place or into the list `out` (same lengths and types), and return the norm before.  A norm that is not finite
-    scales nothing (the caller sees it in the result).  norm: a float32 scalar on the device to use instead (the norm over several devices' tensors, say)."""
+    """Scale the tensors by min(1, limit / norm), in place or into the list `out` (same lengths and types), and return the norm before.  A NaN or infinity among the
+    values scales nothing, and the result is NaN or infinity.  Finite values are scaled whatever their norm (it is used in 64 bits): the result is infinity for one
+    beyond float32 too.  norm: a float32 scalar on the device to use instead (the norm over several devices' tensors, say); NaN or infinity there scales nothing."""
     tensors = list(tensors)
     if not tensors:
         raise ValueError("tensors: at least one expected")
