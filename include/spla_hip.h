@@ -438,10 +438,10 @@ int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint32_t n_expe
                               const void* d_x, void* d_dw, void* d_workspace, size_t workspace_bytes, void* stream);
 /* global_norm: *d_norm = sqrt of the sum of the squares of all elements of all arrays (h_ lists on the host: addresses, lengths in elements, panel types); squares
  * and sums in 64 bits, *d_norm its rounding: infinity for a norm beyond fp32's largest value.  clip_global_norm: h_out[i] = h_arrays[i] * min(1, limit / norm)
- * (h_out[i] may be h_arrays[i]; no other overlap).  norm_given == 0: the norm is computed, written to *d_norm and used in its 64 bits: a NaN or infinity among the
- * values scales nothing, finite values are scaled whatever their norm, also where *d_norm becomes infinity.  norm_given != 0: *d_norm is the norm to use (of
- * arrays on several devices, say) and is read; NaN and infinity scale nothing, so that a norm beyond fp32 cannot be handed from one call to the next.
- * The workspace (splahip_global_norm_workspace bytes, 8-byte aligned) is not needed when the norm is given. */
+ * (h_out[i] may be h_arrays[i]; no other overlap).  norm_given == 0: the norm is computed, written to *d_norm (which lies in no array) and used in its 64 bits: a NaN or
+ * infinity among the values scales nothing, finite values are scaled whatever their norm, also where *d_norm becomes infinity.  norm_given != 0: *d_norm is the norm to
+ * use (of arrays on several devices, say) and is read; NaN and infinity scale nothing, so that a norm beyond fp32 cannot be handed from one call to the next.
+ * The workspace (memory of its own, splahip_global_norm_workspace bytes, 8-byte aligned) is not needed when the norm is given. */
 size_t splahip_global_norm_workspace(uint32_t n_arrays, const uint64_t* h_lengths);
 int splahip_global_norm(uint32_t n_arrays, const void* const* h_arrays, const uint64_t* h_lengths, const int* h_types, void* d_workspace, size_t workspace_bytes,
                         float* d_norm, void* stream);

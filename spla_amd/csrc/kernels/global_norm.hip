@@ -216,6 +216,11 @@ namespace splahip {
             for_batches_of<kBatch>(n_arrays, src, dst, lengths, types, chunk, f);
     }
 
+    static uint64_t bytes_of(uint64_t length, int type) { return length * (type == SPLAHIP_PANEL_FLOAT ? 4u : 2u); }
+    static bool     overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+        return (uintptr_t) a < (uintptr_t) b + b_bytes && (uintptr_t) b < (uintptr_t) a + a_bytes;
+    }
+
     static int check_arrays(uint32_t n_arrays, const void* const* ptrs, const uint64_t* lengths, const int* types) {
         SPLAHIP_REQUIRE(n_arrays == 0 || (ptrs && lengths && types), "null list");
         uint64_t total = 0;
@@ -229,16 +234,24 @@ namespace splahip {
         return SPLAHIP_OK;
     }
 
+    // the partial sums are written while the arrays are read, the norm behind them
+    static int check_workspace(uint32_t n_arrays, const void* const* ptrs, const uint64_t* lengths, const int* types, const void* work, uint64_t work_bytes, const float* norm) {
+        SPLAHIP_REQUIRE(!overlap(norm, sizeof(float), work, work_bytes), "the norm lies inside the workspace");
+        for (uint32_t i = 0; i < n_arrays; ++i) SPLAHIP_REQUIRE(!lengths[i] || !overlap(ptrs[i], bytes_of(lengths[i], types[i]), work, work_bytes), "an array overlaps the workspace");
+        return SPLAHIP_OK;
+    }
+
     // no two results may share memory, and a result may share it with its own source only, element for element: anything else would be scaled twice or read
-    // after it was scaled
-    static int check_overlap(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types, const float* norm) {
+    // after it was scaled.  A norm that is computed (`written`) may not lie inside a source either, which is read again after it was written.
+    static int check_overlap(uint32_t n_arrays, const void* const* src, void* const* dst, const uint64_t* lengths, const int* types, const float* norm,
+                             bool written) {
         struct Span {
             uintptr_t a, b;
             uint32_t  i;
         };
         std::vector<Span> out;
         out.reserve(n_arrays);
-        auto span = [&](const void* p, uint32_t i) { return Span{(uintptr_t) p, (uintptr_t) p + lengths[i] * (types[i] == SPLAHIP_PANEL_FLOAT ? 4u : 2u), i}; };
+        auto span = [&](const void* p, uint32_t i) { return Span{(uintptr_t) p, (uintptr_t) p + bytes_of(lengths[i], types[i]), i}; };
         for (uint32_t i = 0; i < n_arrays; ++i)
             if (lengths[i]) out.push_back(span(dst[i], i));
         std::sort(out.begin(), out.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
@@ -251,6 +264,7 @@ namespace splahip {
         for (uint32_t i = 0; i < n_arrays; ++i) {
             if (lengths[i] == 0 || src[i] == dst[i]) continue;// (its own result: the check above covers the others)
             const Span x = span(src[i], i);
+            SPLAHIP_REQUIRE(!written || !overlap(norm, sizeof(float), src[i], x.b - x.a), "the norm lies inside an array");
             SPLAHIP_REQUIRE(free_of_results(x.a, x.b), "an array overlaps a result other than itself");
         }
         return SPLAHIP_OK;
@@ -272,6 +286,7 @@ extern "C" int splahip_global_norm(uint32_t n_arrays, const void* const* h_array
     if (int st = check_arrays(n_arrays, h_arrays, h_lengths, h_types)) return st;
     SPLAHIP_REQUIRE(d_norm, "null result");
     SPLAHIP_REQUIRE(d_workspace && ((uintptr_t) d_workspace & 7u) == 0 && workspace_bytes >= splahip_global_norm_workspace(n_arrays, h_lengths), "workspace too small");
+    if (int st = check_workspace(n_arrays, h_arrays, h_lengths, h_types, d_workspace, splahip_global_norm_workspace(n_arrays, h_lengths), d_norm)) return st;
     if (int st = ensure_device()) return st;
     hipStream_t    s        = as_stream(stream);
     double*        norm64   = static_cast<double*>(d_workspace);
@@ -295,8 +310,10 @@ extern "C" int splahip_clip_global_norm(uint32_t n_arrays, const void* const* h_
     SPLAHIP_REQUIRE(n_arrays == 0 || h_out, "null list");
     for (uint32_t i = 0; i < n_arrays; ++i) SPLAHIP_REQUIRE(h_lengths[i] == 0 || h_out[i], "null array");
     try {
-        if (int st = check_overlap(n_arrays, h_arrays, h_out, h_lengths, h_types, d_norm)) return st;
+        if (int st = check_overlap(n_arrays, h_arrays, h_out, h_lengths, h_types, d_norm, !norm_given)) return st;
     } catch (const std::bad_alloc&) { return fail(SPLAHIP_ERROR, "out of host memory"); }
+    if (!norm_given && h_out != h_arrays && d_workspace)// (the 64-bit norm is read from there while the results are written)
+        if (int st = check_workspace(n_arrays, h_out, h_lengths, h_types, d_workspace, splahip_global_norm_workspace(n_arrays, h_lengths), d_norm)) return st;
     if (!norm_given)
         if (int st = splahip_global_norm(n_arrays, h_arrays, h_lengths, h_types, d_workspace, workspace_bytes, d_norm, stream)) return st;
     if (int st = ensure_device()) return st;

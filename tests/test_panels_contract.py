@@ -1,0 +1,44 @@
+"""Refusals of the panel operators that their formulas do not show: calls whose results would be wrong or would lose something without a word."""
+import ctypes as C
+
+import pytest
+import torch
+
+from spla_amd import _lib
+
+INVALID = 6
+BASE = 1 << 40  # addresses that nothing reads: the checks come first
+
+
+def _clip(src, dst, lengths, types, norm, given=0):
+    k, work = len(src), (C.c_uint64 * 4096)()
+    with pytest.raises(_lib.SplaHipError) as e:
+        _lib.call("splahip_clip_global_norm", k, (C.c_void_p * k)(*src), (C.c_void_p * k)(*dst), (C.c_uint64 * k)(*lengths), (C.c_int * k)(*types), 1.0, given,
+                  C.cast(work, C.c_void_p), 4096 * 8, C.c_void_p(norm), None)
+    return e.value.status
+
+
+@pytest.mark.parametrize("at", [0, 4, 12])
+def test_the_norm_may_not_be_written_into_an_array_that_is_still_to_be_scaled(at):
+    """the results lie elsewhere, but the norm is written between the pass that sums and the one that scales"""
+    assert _clip([BASE], [BASE + 4096], [4], [0], BASE + at) == INVALID
+    assert _clip([BASE + 8192, BASE], [BASE + 16384, BASE + 4096], [4, 8], [0, 2], BASE + at) == INVALID
+
+
+def test_the_workspace_is_no_array_and_no_norm():
+    """partial sums are written while the arrays are read, and the norm in 64 bits is read while the results are written"""
+    one, n, t = (C.c_void_p * 1), (C.c_uint64 * 1)(100), (C.c_int * 1)(0)
+    need = _lib.call("splahip_global_norm_workspace", 1, n)
+
+    def fails(name, *args):
+        with pytest.raises(_lib.SplaHipError) as e:
+            _lib.call(name, *args)
+        assert e.value.status == INVALID, e.value
+
+    far = C.c_void_p(BASE + (1 << 30))
+    for array in (BASE, BASE + need - 4, BASE - 396):
+        fails("splahip_global_norm", 1, one(array), n, t, C.c_void_p(BASE), need, far, None)
+        fails("splahip_clip_global_norm", 1, one(BASE + (1 << 20)), one(array), n, t, 1.0, 0, C.c_void_p(BASE), need, far, None)
+        fails("splahip_clip_global_norm", 1, one(array), one(array), n, t, 1.0, 0, C.c_void_p(BASE), need, far, None)
+    for norm in (BASE, BASE + need - 4):
+        fails("splahip_global_norm", 1, one(BASE + (1 << 20)), n, t, C.c_void_p(BASE), need, C.c_void_p(norm), None)
