@@ -8,8 +8,11 @@ from __future__ import annotations
 
 import ctypes as C
 from array import array
+from operator import attrgetter
+from types import SimpleNamespace
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import binop_id, scalar_bits, selop_id, type_id
@@ -251,7 +254,8 @@ def mxm(t, a_rows, b_cols, A, B, op_mult, op_add, init, block_products=0, adopt=
 
 # ---- panels: products with a routing matrix, the experts' products, the norm over many tensors --------------------------------------------------------------
 # A panel is a contiguous 2-D tensor [rows, width] of float32, float16 or bfloat16.  The calls are asynchronous on the current stream of the tensors' device,
-# record no autograd graph (the gradients have calls of their own) and can be captured into a graph.
+# record no autograd graph (the gradients have calls of their own) and can be captured into a graph.  An operand whose gradient would be lost by that (it requires
+# one while gradients are recorded, or carries a forward-mode tangent) is refused: such calls belong under torch.no_grad() or into an autograd.Function.
 
 _PANEL_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -276,12 +280,28 @@ def _launch(device, name, *args):
         raise _lib.SplaHipError(status, _lib.load().splahip_last_error().decode(errors="replace"))
 
 
+_requires_grad = attrgetter("requires_grad")
+_forward_recorded = getattr(torch._C, "_is_fwd_grad_enabled", lambda: True)
+_forward = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)  # (below 0: no tangents anywhere; saves the look at each tensor)
+
+
+def _has_tangent(t):
+    return _forward_recorded() and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _differentiated(t):
+    return t.requires_grad and torch.is_grad_enabled() or _forward._current_level >= 0 and _has_tangent(t)
+
+
 def _checked(name, t, dtype, shape, device=None):
-    """t is a contiguous tensor on the GPU of this type, shape and device, else ValueError; returns its address"""
-    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.is_cuda and (device is None or t.device == device) and t.is_contiguous():
+    """t is a contiguous tensor on the GPU of this type, shape and device, and no gradient of it is asked for, else ValueError; returns its address"""
+    if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.is_cuda and (device is None or t.device == device) and t.is_contiguous()
+            and not (t.requires_grad and _differentiated(t)) and (_forward._current_level < 0 or not _has_tangent(t))):
         return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: a tensor expected, not {type(t).__name__}")
+    if _differentiated(t):
+        raise ValueError(f"{name}: its gradient would be lost, since the call records no autograd graph: call it under torch.no_grad() or in an autograd.Function, or detach the tensor")
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} expected, not {t.dtype} of {tuple(t.shape)}")
     if not t.is_cuda or (device is not None and t.device != device):
@@ -438,6 +458,7 @@ def _arrays(name, tensors):
         types = _Words("i", [_PANEL_TYPE[t.dtype] for t in tensors])
         places = set(map(torch.Tensor.get_device, tensors))
         fits = len(places) == 1 and places.pop() >= 0 and all(map(torch.Tensor.is_contiguous, tensors))
+        fits = fits and not (torch.is_grad_enabled() and any(map(_requires_grad, tensors))) and not (_forward._current_level >= 0 and any(map(_has_tangent, tensors)))
     except (AttributeError, KeyError, TypeError):
         fits = False
     if not fits:  # say which

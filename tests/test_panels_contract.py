@@ -3,8 +3,9 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from spla_amd import _lib
+from spla_amd import _lib, kernels
 
 INVALID = 6
 BASE = 1 << 40  # addresses that nothing reads: the checks come first
@@ -42,3 +43,36 @@ def test_the_workspace_is_no_array_and_no_norm():
         fails("splahip_clip_global_norm", 1, one(array), one(array), n, t, 1.0, 0, C.c_void_p(BASE), need, far, None)
     for norm in (BASE, BASE + need - 4):
         fails("splahip_global_norm", 1, one(BASE + (1 << 20)), n, t, C.c_void_p(BASE), need, C.c_void_p(norm), None)
+
+
+def _plan(rows=4, k=2, experts=3):
+    plan = kernels.RoutePlan.__new__(kernels.RoutePlan)  # a plan of CPU tensors: what the checks look at, without a GPU
+    return plan._set(torch.zeros(experts + 1, dtype=torch.int32), torch.zeros(rows * k, dtype=torch.int32), torch.zeros(rows, k, dtype=torch.int32))
+
+
+# operands that have a gradient and are looked at first, with the call that they go into: call(plan, operand), the operand's shape
+OPERANDS = [
+    (lambda p, t: kernels.route_rows(p, t), (4, 8)),
+    (lambda p, t: kernels.route_back(p, t), (8, 8)),
+    (lambda p, t: kernels.route_back_grad(p, t, torch.ones(4, 2), torch.ones(4, 8)), (8, 8)),
+    (lambda p, t: kernels.expert_product(p, torch.ones(8, 5), t), (3, 7, 5)),
+    (lambda p, t: kernels.expert_product_grad(p, torch.ones(8, 5), t, torch.ones(8, 7)), (3, 7, 5)),
+    (lambda p, t: kernels.global_norm([t, torch.ones(2)]), (6,)),
+    (lambda p, t: kernels.clip_global_norm([t, torch.ones(2)], 1.0), (6,)),
+]
+
+
+@pytest.mark.parametrize("call,shape", OPERANDS)
+def test_an_operand_whose_gradient_would_be_lost_is_refused(call, shape, monkeypatch):
+    monkeypatch.setattr(kernels, "_launch", lambda *a: pytest.fail("launched"))
+    with pytest.raises(ValueError, match="gradient"):
+        call(_plan(), torch.ones(shape, requires_grad=True))
+    with pytest.raises(ValueError, match="gradient"):
+        call(_plan(), torch.nn.Parameter(torch.ones(shape)))
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="gradient"):
+        call(_plan(), forward_ad.make_dual(torch.ones(shape), torch.ones(shape)))
+    # with nothing to lose the next thing that is wrong here is said: these are not on the GPU
+    with torch.no_grad(), pytest.raises(ValueError, match="on the GPU|on cpu"):
+        call(_plan(), torch.ones(shape, requires_grad=True))
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="on the GPU|on cpu"):
+        call(_plan(), torch.ones(shape))

@@ -30,3 +30,73 @@ def test_a_given_norm_that_is_not_finite_scales_nothing(dtype, bad):
     kept = [x.clone() for x in t]
     kernels.clip_global_norm(t, 0.25, norm=torch.tensor(bad, device="cuda"))
     assert all(torch.equal(a, b) for a, b in zip(t, kept))
+
+
+def _layer():
+    e = torch.tensor([[0, 1], [2, 0], [1, 1], [-1, 2]], dtype=torch.int32, device="cuda")
+    plan = kernels.route_sort(e, 3)
+    ones = lambda *shape: torch.ones(*shape, device="cuda")  # noqa: E731
+    return plan, ones
+
+
+CALLS = {  # every operand that has a gradient: (plan, operand, ones) -> call, shape
+    "rows x": (lambda p, t, o: kernels.route_rows(p, t), (4, 8)),
+    "rows weights": (lambda p, t, o: kernels.route_rows(p, o(4, 8), t), (4, 2)),
+    "back y": (lambda p, t, o: kernels.route_back(p, t), (8, 8)),
+    "back weights": (lambda p, t, o: kernels.route_back(p, o(8, 8), t), (4, 2)),
+    "back_grad y": (lambda p, t, o: kernels.route_back_grad(p, t, o(4, 2), o(4, 8)), (8, 8)),
+    "back_grad weights": (lambda p, t, o: kernels.route_back_grad(p, o(8, 8), t, o(4, 8)), (4, 2)),
+    "back_grad dout": (lambda p, t, o: kernels.route_back_grad(p, o(8, 8), o(4, 2), t), (4, 8)),
+    "product x": (lambda p, t, o: kernels.expert_product(p, t, o(3, 7, 5)), (8, 5)),
+    "product w": (lambda p, t, o: kernels.expert_product(p, o(8, 5), t), (3, 7, 5)),
+    "product_grad x": (lambda p, t, o: kernels.expert_product_grad(p, t, o(3, 7, 5), o(8, 7)), (8, 5)),
+    "product_grad w": (lambda p, t, o: kernels.expert_product_grad(p, o(8, 5), t, o(8, 7)), (3, 7, 5)),
+    "product_grad dy": (lambda p, t, o: kernels.expert_product_grad(p, o(8, 5), o(3, 7, 5), t), (8, 7)),
+    "norm": (lambda p, t, o: kernels.global_norm([o(2), t]), (6,)),
+    "clip": (lambda p, t, o: kernels.clip_global_norm([o(2), t], 1.0), (6,)),
+    "clip out": (lambda p, t, o: kernels.clip_global_norm([o(2), o(6)], 1.0, out=[o(2), t]), (6,)),
+    "clip norm": (lambda p, t, o: kernels.clip_global_norm([o(2)], 1.0, norm=t), ()),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_an_operand_whose_gradient_would_be_lost_is_refused(name):
+    call, shape = CALLS[name]
+    plan, ones = _layer()
+    tracked = torch.ones(shape, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        call(plan, tracked, ones)
+    with pytest.raises(ValueError, match="gradient"):
+        call(plan, tracked * 1, ones)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(ValueError, match="gradient"):
+        call(plan, torch.autograd.forward_ad.make_dual(torch.ones(shape, device="cuda"), torch.ones(shape, device="cuda")), ones)
+    with pytest.raises(Exception):  # a batched tensor has no memory of its own
+        torch.vmap(lambda t: call(plan, t, ones))(torch.ones(2, *shape, device="cuda"))
+    # nothing to lose
+    call(plan, tracked.detach(), ones)
+    with torch.no_grad():
+        call(plan, tracked, ones)
+    with torch.autograd.forward_ad.dual_level():
+        call(plan, torch.ones(shape, device="cuda"), ones)
+
+
+def test_inside_an_autograd_function():
+    """the way that a training program has the gradients: forward and backward call the operators, nothing is recorded inside"""
+    class Product(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w, plan):
+            ctx.plan = plan
+            ctx.save_for_backward(x, w)
+            return kernels.expert_product(plan, x, w)
+
+        @staticmethod
+        def backward(ctx, dy):
+            return (*kernels.expert_product_grad(ctx.plan, *ctx.saved_tensors, dy.contiguous()), None)
+
+    plan, ones = _layer()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, w = (torch.randint(-3, 4, s, generator=g, device="cuda").float().requires_grad_() for s in ((8, 5), (3, 7, 5)))
+    factor = torch.randint(-3, 4, (8, 7), generator=g, device="cuda").float()
+    (Product.apply(x, w, plan) * factor).sum().backward()
+    dx, dw = kernels.expert_product_grad(plan, x.detach(), w.detach(), factor)
+    assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw) and dx.any() and dw.any()
