@@ -507,4 +507,5 @@ def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None)
         work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
     _launch(device, "splahip_clip_global_norm", len(tensors), ptrs.ptr, out_ptrs.ptr, lengths.ptr, types.ptr, float(limit), given, work.data_ptr() if work is not None else None,
             n_bytes, norm.data_ptr())
+    torch.autograd.graph.increment_version(tensors if out is None else out)  # (a graph that kept one of them for its backward pass notices)
     return norm

@@ -100,3 +100,32 @@ def test_inside_an_autograd_function():
     (Product.apply(x, w, plan) * factor).sum().backward()
     dx, dw = kernels.expert_product_grad(plan, x.detach(), w.detach(), factor)
     assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw) and dx.any() and dw.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clipping_is_seen_by_a_graph_that_kept_the_tensor(dtype):
+    """as any change in place: a backward pass over values that are no longer there raises instead of using the new ones"""
+    w = torch.ones(9, device="cuda", dtype=dtype, requires_grad=True)
+    kept, out = (torch.full((9,), 3.0, device="cuda", dtype=dtype) for _ in range(2))
+    loss = (kept * w).sum()
+    kernels.clip_global_norm([kept], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    bucket = torch.zeros(64, device="cuda", dtype=dtype)
+    loss = (out * w).sum() + (bucket[32:41] * w).sum()
+    before = [t._version for t in (kept, out, bucket)]
+    kernels.clip_global_norm([kept, kept], 1.0, out=[out, bucket[32:41]])
+    assert [t._version - b for t, b in zip((kept, out, bucket), before)] == [0, 1, 1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    loss = (kept * w).sum()
+    kernels.global_norm([kept])
+    loss.backward()  # reading changes nothing
+
+
+def test_clipping_tensors_of_inference_mode():
+    with torch.inference_mode():
+        t = torch.full((4,), 2.0, device="cuda")
+        kernels.clip_global_norm([t], 1.0)
+    kernels.clip_global_norm([t], 0.5)
+    assert t.tolist() == [0.25] * 4
