@@ -280,7 +280,7 @@ def _launch(device, name, *args):
         raise _lib.SplaHipError(status, _lib.load().splahip_last_error().decode(errors="replace"))
 
 
-_requires_grad = attrgetter("requires_grad")
+_requires_grad, _is_neg = attrgetter("requires_grad"), torch.Tensor.is_neg
 _forward_recorded = getattr(torch._C, "_is_fwd_grad_enabled", lambda: True)
 _forward = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)  # (below 0: no tangents anywhere; saves the look at each tensor)
 
@@ -296,12 +296,14 @@ def _differentiated(t):
 def _checked(name, t, dtype, shape, device=None):
     """t is a contiguous tensor on the GPU of this type, shape and device, and no gradient of it is asked for, else ValueError; returns its address"""
     if (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.is_cuda and (device is None or t.device == device) and t.is_contiguous()
-            and not (t.requires_grad and _differentiated(t)) and (_forward._current_level < 0 or not _has_tangent(t))):
+            and not t.is_neg() and not (t.requires_grad and _differentiated(t)) and (_forward._current_level < 0 or not _has_tangent(t))):
         return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: a tensor expected, not {type(t).__name__}")
     if _differentiated(t):
         raise ValueError(f"{name}: its gradient would be lost, since the call records no autograd graph: call it under torch.no_grad() or in an autograd.Function, or detach the tensor")
+    if t.is_neg():
+        raise ValueError(f"{name}: its values are those of its memory negated: resolve_neg() expected")
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} expected, not {t.dtype} of {tuple(t.shape)}")
     if not t.is_cuda or (device is not None and t.device != device):
@@ -493,6 +495,9 @@ def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None)
     out_ptrs = ptrs
     if out is not None:
         out = list(out)
+        for name, list_ in (("tensors", tensors), ("out", out)):  # (in place the sign stays with the tensor, and the norm does not see it)
+            if any(map(_is_neg, list_)):
+                raise ValueError(f"{name}: the values of one are those of its memory negated: resolve_neg() expected")
         if len(out) != len(tensors):
             raise ValueError(f"out: {len(tensors)} tensors expected, not {len(out)}")
         out_ptrs, out_lengths, out_types, out_device = _arrays("out", out)

@@ -76,3 +76,18 @@ def test_an_operand_whose_gradient_would_be_lost_is_refused(call, shape, monkeyp
         call(_plan(), torch.ones(shape, requires_grad=True))
     with forward_ad.dual_level(), pytest.raises(ValueError, match="on the GPU|on cpu"):
         call(_plan(), torch.ones(shape))
+
+
+NEGATED = OPERANDS[:5] + [
+    (lambda p, t: kernels.clip_global_norm([t], 1.0, out=[torch.ones(6)]), (6,)),
+]
+
+
+@pytest.mark.parametrize("call,shape", NEGATED)
+def test_a_tensor_that_negates_its_memory_is_refused(call, shape, monkeypatch):
+    """the imaginary part of a conjugate, say: its values are its memory's with the other sign, which a call that takes the address would not see"""
+    monkeypatch.setattr(kernels, "_launch", lambda *a: pytest.fail("launched"))
+    with pytest.raises(ValueError, match="negat"):
+        call(_plan(), torch._neg_view(torch.ones(shape)))
+    one = torch.ones(1, 1, dtype=torch.complex64).conj().imag
+    assert one.is_contiguous() and one.is_neg()

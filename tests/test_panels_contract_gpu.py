@@ -129,3 +129,18 @@ def test_clipping_tensors_of_inference_mode():
         kernels.clip_global_norm([t], 1.0)
     kernels.clip_global_norm([t], 0.5)
     assert t.tolist() == [0.25] * 4
+
+
+def test_tensors_that_negate_their_memory():
+    """refused where the sign would be lost; the norm does not see it, and scaling in place keeps it"""
+    plan, ones = _layer()
+    negated = lambda *shape: torch._neg_view(ones(*shape))  # noqa: E731
+    for call in (lambda: kernels.route_rows(plan, ones(4, 8), negated(4, 2)), lambda: kernels.route_back_grad(plan, ones(8, 8), ones(4, 2), negated(4, 8)),
+                 lambda: kernels.expert_product(plan, negated(8, 5), ones(3, 7, 5)), lambda: kernels.clip_global_norm([negated(4)], 1.0, out=[ones(4)]),
+                 lambda: kernels.clip_global_norm([ones(4)], 1.0, out=[negated(4)])):
+        with pytest.raises(ValueError, match="negat"):
+            call()
+    t = negated(4)
+    assert float(kernels.global_norm([t])) == 2.0
+    kernels.clip_global_norm([t], 1.0)
+    assert t.tolist() == [-0.5] * 4
