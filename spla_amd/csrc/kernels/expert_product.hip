@@ -206,21 +206,24 @@ namespace splahip {
     __device__ const uint4 zero_page[4] = {};
 
     // One load per lane into LDS at dst + (16 or 4) lane, dst the same for the whole wavefront.  Assembly, because the compiler waits for every such load before the next LDS
-    // read of any address; the kernel waits itself, by loads_arrived().  There is no result register that the compiler could reuse early.  (M0 holds dst; the
-    // compiler sets it anew wherever it needs it.  Five wait states lie between whatever may have made `base` - a read of a lane is vector work - and the load, which the
-    // compiler sees to for its own instructions only.)
+    // read of any address; the kernel waits itself, by loads_arrived().  There is no result register that the compiler could reuse early.  M0 holds dst
+    // and is named as changed, so that the compiler keeps nothing there across it (it warns that M0 is reserved, which is meant).  Five wait states lie between
+    // whatever may have made `base` - a read of a lane is vector work - and the load, which the compiler sees to for its own instructions only.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
     template<Load LOAD>
     __device__ __forceinline__ void load_to_lds(const void* src, uint32_t dst) {
-        if constexpr (LOAD == kUnits) asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+        if constexpr (LOAD == kUnits) asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
         else
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, off" ::"s"(dst), "v"(src) : "memory", "m0");
     }
     template<Load LOAD>
     __device__ __forceinline__ void load_to_lds_at(const void* base, uint32_t offset, uint32_t dst) {
-        if constexpr (LOAD == kUnits) asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+        if constexpr (LOAD == kUnits) asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory", "m0");
         else
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(offset), "s"(base) : "memory", "m0");
     }
+#pragma clang diagnostic pop
     template<uint32_t LEFT>
     __device__ __forceinline__ void loads_arrived() {// all but the last LEFT of this wavefront's loads (and stores) into memory order
         static_assert(LEFT < 64, "a six-bit counter");
