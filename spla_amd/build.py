@@ -51,7 +51,8 @@ def _compile(src: Path, force: bool, hdr_mtime: float) -> Path:
         return obj
     cmd = [HIPCC, *COMMON]
     if src.suffix == ".hip":
-        # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then (the host pass does not know the feature and says so)
+        # no packed fp32 arithmetic, a precaution: its forms are not trusted on this hardware, and scalar ones cost the sparse products nothing that could be measured
+        # (453.1 and 453.9 GTEPS, both in turn).  The host pass does not know the feature and says so.  jit.hip gives its compiler the same switch.
         cmd += [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     else:
         cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include"]

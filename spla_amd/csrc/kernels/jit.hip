@@ -470,8 +470,9 @@ namespace {
             std::string name = prop.gcnArchName;
             arch             = "--offload-arch=" + name.substr(0, name.find(':'));
         }
-        const char*  opts[] = {arch.c_str(), "-O3", "-ffp-contract=off"};
-        hiprtcResult cr     = r.CompileProgram(prog, 3, opts);
+        // (no packed fp32 arithmetic, like the library's own kernels)
+        const char*  opts[] = {arch.c_str(), "-O3", "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"};
+        hiprtcResult cr     = r.CompileProgram(prog, (int) (sizeof opts / sizeof *opts), opts);
         if (cr != HIPRTC_SUCCESS) {
             size_t      n = 0;
             std::string log;

@@ -37,3 +37,18 @@ def test_assembly_that_writes_m0_says_so(path):
 def test_the_rule_finds_the_statements():
     text = 'asm volatile("s_mov_b32 m0, %0" ::"s"(f(x)) : "memory");  asm("" : "+v"(y));  asm volatile("s_nop 3")'
     assert list(_assembly(text)) == [('"s_mov_b32 m0, %0" ', '::"s"(f(x)) : "memory")'), ('"" ', ': "+v"(y))'), ('"s_nop 3")', "")]
+
+
+SWITCH = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def _strings(text):
+    return re.findall(r'"((?:\\.|[^"\\])*)"', text)
+
+
+def test_both_compilers_build_without_packed_fp32_arithmetic():
+    """the library's kernels (build.py) and the ones around user-defined ops, which are compiled at run time (jit.hip)"""
+    ahead = _strings(re.search(r"cmd \+= \[f\"--offload-arch=.*?\]", (CSRC.parent / "build.py").read_text()).group())
+    at_run_time = _strings(re.search(r"opts\[\]\s*=\s*\{.*?\};", (CSRC / "kernels" / "jit.hip").read_text(), re.S).group())
+    assert ahead[-4:] == SWITCH
+    assert at_run_time[-4:] == SWITCH

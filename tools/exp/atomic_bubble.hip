@@ -7,7 +7,7 @@
 //   A = 3 agent scope, returning, an address per wave (no contention)        A = 4 agent scope, NOT returning, shared address
 //   A = 6 system scope, returning, one address per 16 workgroups
 //   A = 7 / 8 no atomic, but every wave walks its own span / 8 KB runs (what a wave-level claim makes of the stream) instead of the workgroup's waves side by side, 1 KB each
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/exp/bin/atomic_bubble tools/exp/atomic_bubble.hip
+// build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o tools/exp/bin/atomic_bubble tools/exp/atomic_bubble.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>

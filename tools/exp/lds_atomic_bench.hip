@@ -1,5 +1,5 @@
 // LDS atomic throughput on gfx950: ds_add_f32 / ds_add_u32 / ds_min_i32 / plain RMW / plain store, by address pattern.
-// Build: hipcc --offload-arch=gfx950 -O3 -o tools/exp/bin/lds_atomic_bench tools/exp/lds_atomic_bench.hip
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o tools/exp/bin/lds_atomic_bench tools/exp/lds_atomic_bench.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

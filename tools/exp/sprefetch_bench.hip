@@ -3,7 +3,7 @@
 // L2 when the vector load asks for it leaves its slot sooner.  Round 3's attempt faulted on an out-of-range address and was never measured.)
 //   every streaming wave issues, beside the 16-byte vector loads of its step, one s_load_dword per 128-byte line of the data it will read A steps later (no wait: the
 //   results are never used); at most 15 scalar loads are outstanding per wave (lgkmcnt), so the prefetch throttles itself
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/exp/bin/sprefetch_bench tools/exp/sprefetch_bench.hip
+// build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o tools/exp/bin/sprefetch_bench tools/exp/sprefetch_bench.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>

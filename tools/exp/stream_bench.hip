@@ -7,7 +7,7 @@
 //   C  scalar-cache prefetch: one wave per workgroup walks the stream ahead of the vector loads with s_load_dwordx2 per 128-byte line
 //      (does a line pulled through the scalar cache's path land in L2 early enough to shorten the vector loads' stay in the L1's miss queue?)
 //
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/exp/bin/stream_bench tools/exp/stream_bench.hip
+// build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -o tools/exp/bin/stream_bench tools/exp/stream_bench.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
