@@ -261,8 +261,10 @@ _PANEL_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 _entries = {}
-# the current stream's handle and device without the Python objects and checks around them (a fifth of a small call's time; the tensors have initialised the GPU)
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# the current stream's handle and device without the Python objects and checks around them (a fifth of a small call's time; the tensors have initialised the GPU), where
+# torch has these
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _launch(device, name, *args):

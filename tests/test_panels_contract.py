@@ -1,5 +1,8 @@
 """Refusals of the panel operators that their formulas do not show: calls whose results would be wrong or would lose something without a word."""
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -91,3 +94,20 @@ def test_a_tensor_that_negates_its_memory_is_refused(call, shape, monkeypatch):
         call(_plan(), torch._neg_view(torch.ones(shape)))
     one = torch.ones(1, 1, dtype=torch.complex64).conj().imag
     assert one.is_contiguous() and one.is_neg()
+
+
+def test_the_module_loads_without_private_parts_of_torch():
+    """the sparse operators of the same module need none of what the panel operators save time with"""
+    program = """
+import torch
+for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice", "_is_fwd_grad_enabled"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+if hasattr(torch.autograd.forward_ad, "_current_level"):
+    del torch.autograd.forward_ad._current_level
+from spla_amd import kernels
+assert callable(kernels.mxv_masked) and callable(kernels.route_sort)
+print("loaded")
+"""
+    run = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "loaded" in run.stdout, run.stderr

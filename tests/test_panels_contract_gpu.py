@@ -1,4 +1,6 @@
 """What the documentation of the panel operators says beyond their formulas, on the GPU."""
+import importlib.util
+
 import pytest
 import torch
 
@@ -144,3 +146,33 @@ def test_tensors_that_negate_their_memory():
     assert float(kernels.global_norm([t])) == 2.0
     kernels.clip_global_norm([t], 1.0)
     assert t.tolist() == [-0.5] * 4
+
+
+def test_the_current_stream_by_public_calls(monkeypatch):
+    """a copy of the module that found no private shortcuts: the same results, on a side stream and inside a graph"""
+    spec = importlib.util.spec_from_file_location("spla_amd.kernels_without_shortcuts", kernels.__file__)
+    copy = importlib.util.module_from_spec(spec)
+    with monkeypatch.context() as m:
+        for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+            m.delattr(torch._C, name)
+        spec.loader.exec_module(copy)
+    assert copy._raw_stream is not kernels._raw_stream and copy._current_device is not kernels._current_device
+    e = torch.randint(-1, 5, (700, 2), dtype=torch.int32, device="cuda")
+    x = torch.randn(700, 64, device="cuda")
+    want = kernels.route_rows(kernels.route_sort(e, 5), x)
+    side = torch.cuda.Stream()
+    assert copy._raw_stream(0) == torch.cuda.current_stream().cuda_stream == kernels._raw_stream(0) and copy._current_device() == kernels._current_device()
+    with torch.cuda.stream(side):
+        assert copy._raw_stream(0) == side.cuda_stream == kernels._raw_stream(0)
+        side.wait_stream(torch.cuda.default_stream())
+        got = copy.route_rows(copy.route_sort(e, 5), x)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = copy.route_rows(copy.route_sort(e, 5), x)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
