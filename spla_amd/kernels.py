@@ -257,6 +257,7 @@ def mxm(t, a_rows, b_cols, A, B, op_mult, op_add, init, block_products=0, adopt=
 # record no autograd graph (the gradients have calls of their own) and can be captured into a graph.  An operand whose gradient would be lost by that (it requires
 # one while gradients are recorded, or carries a forward-mode tangent) is refused: such calls belong under torch.no_grad() or into an autograd.Function.
 
+_LARGEST = torch.finfo(torch.float32).max
 _PANEL_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -309,7 +310,7 @@ def _checked(name, t, dtype, shape, device=None):
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name}: {dtype} of shape {tuple(shape)} expected, not {t.dtype} of {tuple(t.shape)}")
     if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{name}: a tensor on {device or 'the GPU'} expected, not on {t.device}")
+        raise ValueError(f"{name}: a tensor on {device if t.is_cuda else 'the GPU'} expected, not on {t.device}")
     raise ValueError(f"{name}: a contiguous tensor expected, not one of strides {t.stride()}")
 
 
@@ -490,9 +491,11 @@ def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None)
     """Scale the tensors by min(1, limit / norm), in place or into the list `out` (same lengths and types), and return the norm before.  A NaN or infinity among the
     values scales nothing, and the result is NaN or infinity.  Finite values are scaled whatever their norm (it is used in 64 bits): the result is infinity for one
     beyond float32 too.  norm: a float32 scalar on the device to use instead (the norm over several devices' tensors, say); NaN or infinity there scales nothing."""
-    tensors = list(tensors)
+    tensors, limit = list(tensors), float(limit)
     if not tensors:
         raise ValueError("tensors: at least one expected")
+    if not 0.0 <= limit <= _LARGEST:
+        raise ValueError(f"limit: a largest norm of 0 or more that float32 holds expected, not {limit}")
     ptrs, lengths, types, device = _arrays("tensors", tensors)
     out_ptrs = ptrs
     if out is not None:
@@ -512,7 +515,7 @@ def clip_global_norm(tensors, limit: float, out=None, norm: torch.Tensor = None)
         norm = torch.empty((), dtype=torch.float32, device=device)
         n_bytes, given = _lib.load().splahip_global_norm_workspace(len(tensors), lengths.ptr), 0
         work = torch.empty(n_bytes, dtype=torch.uint8, device=device)
-    _launch(device, "splahip_clip_global_norm", len(tensors), ptrs.ptr, out_ptrs.ptr, lengths.ptr, types.ptr, float(limit), given, work.data_ptr() if work is not None else None,
+    _launch(device, "splahip_clip_global_norm", len(tensors), ptrs.ptr, out_ptrs.ptr, lengths.ptr, types.ptr, limit, given, work.data_ptr() if work is not None else None,
             n_bytes, norm.data_ptr())
     torch.autograd.graph.increment_version(tensors if out is None else out)  # (a graph that kept one of them for its backward pass notices)
     return norm

@@ -111,3 +111,18 @@ print("loaded")
 """
     run = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "loaded" in run.stdout, run.stderr
+
+
+@pytest.mark.parametrize("limit", [-1.0, -1e-45, float("inf"), float("nan"), 1e39])
+def test_a_limit_that_is_no_largest_norm_is_a_value_error(limit, monkeypatch):
+    """like every argument that the Python face can see to be wrong; before anything is allocated or launched"""
+    monkeypatch.setattr(kernels, "_launch", lambda *a: pytest.fail("launched"))
+    with pytest.raises(ValueError, match="limit"):
+        kernels.clip_global_norm([torch.ones(3)], limit)
+
+
+def test_a_tensor_in_host_memory_is_named_as_such():
+    with pytest.raises(ValueError, match="on the GPU expected, not on cpu"):
+        kernels.global_norm([torch.ones(3)])
+    with pytest.raises(ValueError, match="on the GPU expected, not on cpu"):
+        kernels.route_rows(_plan(), torch.ones(4, 8))
