@@ -871,7 +871,7 @@ extern "C" int splahip_expert_product_dw(int panel_type, uint32_t n_places, uint
     ProductArgs    g{d_dy, d_x, d_dw, n_places, n_experts, n_out, n_in, 0, d_offsets};
     g.splits = matrix_grad_splits(g, element, aligned_product(g, 16 / element));
     if (g.splits == 1) return launch_product<kMatrixGrad>(panel_type, g, s);
-    g.c = d_workspace;// (its alignment does not choose another kernel: the parts are fp32 and stored as such)
+    g.c = d_workspace;// (aligned, so that operands in units take the kernel for units even if d_dw starts between two: both have tiles of the size that g.splits was chosen for)
     if (int st = launch_product<kMatrixGrad>(panel_type, g, s)) return st;
     const uint64_t n = (uint64_t) n_experts * n_in * n_out;
     panel_dispatch(panel_type, [&](auto zero) {
