@@ -426,7 +426,7 @@ int splahip_route_back(int panel_type, uint32_t n_rows, uint32_t per_row, uint32
 int splahip_route_back_grad(int panel_type, uint32_t n_rows, uint32_t per_row, uint32_t n_experts, uint32_t width, const uint32_t* d_offsets, const int32_t* d_place,
                             const float* d_weights, const void* d_y, const void* d_dout, void* d_dy, float* d_dweights, void* stream);
 /* expert_product: with the rows in expert order, d_y[p, :] = d_w[e] d_x[p, :] for p in [d_offsets[e], d_offsets[e + 1]), d_w = [n_experts, n_out, n_in] row-major; the
- * rows behind the last entry become 0 and are not read.  _dx: d_dx[p, :] = d_w[e]^T d_dy[p, :].  _dw: d_dw[e] = sum of d_dy[p, :] d_x[p, :]^T over the expert's
+ * rows behind the last entry become 0, whatever d_x holds there.  _dx: d_dx[p, :] = d_w[e]^T d_dy[p, :].  _dw: d_dw[e] = sum of d_dy[p, :] d_x[p, :]^T over the expert's
  * rows (0 without rows); its workspace (16-byte aligned) takes the sums of parts of the rows where the matrices are too small to fill the card by themselves.
  * fp32 panels are multiplied in full fp32.  n_in, n_out < 2^21. */
 int splahip_expert_product(int panel_type, uint32_t n_places, uint32_t n_experts, uint32_t n_in, uint32_t n_out, const uint32_t* d_offsets, const void* d_x,

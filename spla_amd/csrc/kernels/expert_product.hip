@@ -5,7 +5,7 @@
 //   splahip_expert_product_dx  dx[p, :] = w[e(p)]^T dy[p, :]
 //   splahip_expert_product_dw  dw[e]    = sum over the expert's rows of dy[p, :] x[p, :]^T
 //
-// Rows behind the last entry (offsets[n_experts] ..) become 0; an expert without rows has dw = 0.  fp32 sums in a fixed order, one rounding to the panel's
+// Rows behind the last entry (offsets[n_experts] ..) become 0, and what operands hold there does not count; an expert without rows has dw = 0.  fp32 sums in a fixed order, one rounding to the panel's
 // type.  fp32 panels are multiplied in full fp32 (v_mfma_f32_32x32x2_f32).
 #include "panel.hpp"
 
@@ -198,8 +198,9 @@ namespace splahip {
 
     // ---- from memory to LDS ------------------------------------------------------------------------------------------------------------------------------
     // kUnits: 16 bytes per lane straight into LDS; operands, rows and the result begin at multiples of 16 bytes.
-    // kWords: 4 bytes per lane straight into LDS; fp32 of any sizes (8000 rows x 1001 x 1003 over 8, forward, dx, dw: 168, 162, 144 us; as kElements 267, 226, 160; 4800 rows x
-    // 250 x 333 over 5: 16, 20, 21 us against 21, 24, 22, and 14, 17, 19 as kUnits at 252 x 336).
+    // kWords: 4 bytes per lane straight into LDS; fp32 of any sizes.  4800 rows x 250 x 333 over 5, forward, dx, dw: 15, 18, 19 us, and 13, 16, 18 as kUnits at 252 x 336; as
+    // kElements 1.3, 1.2 and 1.1 times as long, and 1.6, 1.4 and 1.1 times at 8000 rows x 1001 x 1003 over 8 (155, 155, 132 us, random loads).  The lane's addresses cost: the
+    // compiler spills 31 to 144 scalar registers in these kernels.
     // kElements: through registers, 16 bytes per lane from any address, the ends of rows element by element; 16-bit elements of odd sizes or alignment.
     enum Load { kUnits, kWords, kElements };
 
@@ -320,11 +321,12 @@ namespace splahip {
     // instructions run from registers, the operands of the next are read from LDS.  LDS holds five slabs, A0 B0 A1 B1 A2 ..: one barrier per step, before its last
     // quarter: behind it every wavefront has read this step's two slabs, so the next two loads may overwrite them, and the next step's slabs have arrived (issued one
     // step ago, A's two steps ago).  The loads of the next tile's first slabs are under way while a tile's result is stored.
-    // Bound: in 16 bits the card's power.  32768 rows x 2048 x 4096 over 8 even experts, 256 x 256 tiles: 445 us = 1.23 PFLOP/s forward, 435 and 450 for the gradients, at 1.7 GHz
-    // (on zeros, which cost no power, 350 us = 1.57); 128 x 128 tiles 585 us: an operand's byte is used half as often.  fp32: the matrix cores, 8192 x 1024 x 1024 over 8
-    // experts 150 us = 115 TFLOP/s.  kElements at 16384 x 1001 x 1003: 400, 400 and 515 TFLOP/s (forward, dx, dw) where 1000 x 1008
-    // has 650, 650 and 755: its slabs go through registers, with misaligned 16-byte accesses; which of the two costs was not measured apart.
-    // Small problems (4096 x 1024 x 1024 over 16 experts: 20 us) wait for the CUs that have two tiles.
+    // Bound: in 16 bits the card's power.  32768 rows x 2048 x 4096 over 8 even experts, 256 x 256 tiles: 472 us = 1.17 PFLOP/s forward, 442 and 453 for the gradients, at 1.7 GHz
+    // (on zeros, which cost no power, 353 us = 1.56); 128 x 128 tiles 1.3 times as long: an operand's byte is used half as often.  256 x 256 tiles of the forward product and the
+    // row gradient take all 256 vector registers and spill three (16 bytes a lane of scratch).  fp32: the matrix cores, 8192 x 1024 x 1024 over 8 even experts 127 us =
+    // 135 TFLOP/s.  kElements at 16384 x 1001 x 1003 over 8: 560, 590 and 600 TFLOP/s (forward, dx, dw) at even loads, 450, 470 and 590 at random ones, where 1000 x 1008
+    // has 785, 850, 800 and 650, 690, 780: its slabs go through registers, with misaligned 16-byte accesses; which of the two costs was not measured apart.
+    // Small problems (4096 x 1024 x 1024 over 16 experts: 14 us at even loads, 20 at random ones) wait for the CUs that have two tiles.
     //
     // take(tile): the workgroup's next tile, false behind the last.  O: the result's type, T or (partial sums) float
     template<typename T, typename O, Form FORM, Load LOAD, uint32_t BM, uint32_t WM, uint32_t WN, typename TAKE>
@@ -630,9 +632,13 @@ namespace splahip {
     // part of the matrix is read again, from the cache); its WAVES wavefronts take the depth in turns of 128 bytes, so that a matrix row is read in runs of
     // 512 and more, and go from memory to the matrix instruction without LDS: lane l holds row l % 16, 16 bytes of k from unit l / 16.  The wavefronts' sums are joined in LDS in
     // a fixed order.  Many small workgroups instead of a few that stay: what counts is bytes under way.
-    // 256 rows over 32 matrices of 2048 x 2048 bf16, none of it cached: 50 us = 5.4 TB/s (the tile kernel: 64); 2 rows through two of eight 2048 x 4096: 9 us (18).  One row block of
+    // 256 rows over 32 matrices of 2048 x 2048 bf16, none of it cached: 51 us = 5.3 TB/s (the tile kernel: 64); 2 rows through two of eight 2048 x 4096: 9 us with the matrices
+    // in the cache behind the L2s, 11 without (18).  One row block of
     // 16 and 32 columns instead of 64: 61 us (the rows are read too often); through LDS in whole rows: 65.  Where that leaves CUs without work, 16 columns and eight
-    // wavefronts (8 rows through 8 of 13 matrices of 4032 x 192: 14.0 -> 7.7 us).  From 24 rows per expert on the tile kernel is the faster one.
+    // wavefronts (8 rows through 8 of 13 matrices of 4032 x 192: 14.0 -> 7.7 us).
+    // The choice goes by the average of the rows per expert, all that the host knows: up to 24.  Even loads meet there (2048 x 2048 bf16, 768 rows over 32 experts 59 us, the tile
+    // kernel 55 over 31; 1536 over 64: 106, and 124 over 63).  It does not bound uneven ones: an expert's blocks of 32 rows come one after another in one column of
+    // workgroups, so that all rows at one expert take 96 us for 256 rows, 284 for 768 and 565 for 1536, where the tile kernel takes 22.
     __device__ __forceinline__ f32x4 matrix_step16(s16x8 a, s16x8 b, f32x4 c, bf16_t) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
@@ -803,8 +809,7 @@ namespace splahip {
         } else {
             auto tiles = [&](uint64_t bm) { return (g.n_places / bm + 1) * ((g.n + bm - 1) / bm); };
             if constexpr (FORM == kForward)
-                if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts && g.n_experts * (uint64_t) (g.n / 32 + 1) < (1u << 23))// (a launch holds fewer than 2^32 threads)
-{
+                if (aligned && g.n_places <= 24 * (uint64_t) g.n_experts && g.n_experts * (uint64_t) (g.n / 32 + 1) < (1u << 23)) {// (a launch holds fewer than 2^32 threads)
                     const uint64_t rows = std::min(g.n_places, g.n_experts);// experts that have some, at most
                     if (rows * (g.n / 64) >= 1024) return launch_few_rows<T, 4, 4>(g, s);
                     return rows * (g.n / 32) >= 192 ? launch_few_rows<T, 2, 4>(g, s) : launch_few_rows<T, 1, 8>(g, s);

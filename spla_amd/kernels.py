@@ -418,7 +418,7 @@ def _matrices(plan, w, dtype):
 
 def expert_product(plan: RoutePlan, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """y[p] = w[e] @ x[p] for the places p of expert e: x [n_places, n_in] in expert order, w [n_experts, n_out, n_in] of the same type.  Rows behind the last
-    entry are not read and become 0."""
+    entry become 0, whatever x holds there."""
     t = _panel_type("x", x)
     src_w, n_out, n_in = _matrices(plan, w, x.dtype)
     src = _checked("x", x, x.dtype, (plan.n_places, n_in), plan.device)
