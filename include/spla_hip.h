@@ -402,7 +402,8 @@ int splahip_vec_coo_to_dense(uint32_t n, uint32_t nvals, const uint32_t* d_idx, 
  * Operators of a layer of experts and of its training step.  Not in the reference.  A panel is a dense row-major matrix of `panel_type` elements without
  * gaps between its rows.  A router's choice is a matrix of n_rows tokens x n_experts with per_row entries in every row: d_experts[row * per_row + choice]; an
  * expert outside [0, n_experts) is no entry (padding).  n_places = n_rows * per_row.  All calls are asynchronous on `stream`, keep nothing between calls and
- * can be captured into a graph; workspaces are the caller's (one call at a time per workspace).  Sums are kept in fp32 or wider, in a fixed order (the same
+ * can be captured into a graph; workspaces are the caller's (one call at a time per workspace).  Results and
+ * workspaces share no memory with anything else of a call, unless it says so.  Sums are kept in fp32 or wider, in a fixed order (the same
  * result from run to run), and rounded to the panel's type once.  Limits: n_experts <= 2048, n_places < 2^31.
  *
  * route_sort     : the entries sorted by expert, stable (the transpose of the routing matrix): d_offsets[e] = entries with an expert below e (n_experts + 1
